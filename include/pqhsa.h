@@ -406,6 +406,90 @@ int pqhsa_scan_scores_static(const pqhsa_params* p, float* scores, void* stream)
 int pqhsa_topk_radix(const float* scores, int32_t rows, int32_t n, int64_t row_stride, int32_t k,
                      int32_t* out_idx, float* out_val, void* stream);
 
+/* ---- dense attention over a paged cache, and eviction from it ---------------------------------------------------
+ *
+ * The exact form of the decode step for requests that have no index (too short for one, or wanted exact), and the
+ * other way of bounding a long cache: dropping the keys that have gathered the least attention weight.  The reference
+ * has neither: its plugin hands such steps back to the serving engine
+ * (benchmarks/vllm_backend/pq_hsa_decode_runtime.py:790-822).  Same page layouts as above; the lengths, positions and
+ * block tables are read on the device, so every call can be captured in a CUDA graph and replayed as requests grow.
+ *
+ * Request r holds n = seq_lens[r] key slots per KV head.  The position of slot i is i, or key_pos[r, h, i] (after an
+ * eviction, where slots are in no order); query token t of T sits at position p_t = n - T + t, or, with query_pos, at
+ * query_pos[r] - (T - 1) + t.  Token t sees key i at position x when
+ *     first <= x <= p_t  and  (window == 0  or  p_t - x < window  or  x - first < sink_tokens),
+ * first = first_key[r] (0 without: where the request's current document starts).  Its score is
+ *     s = scale <q, k>;  s = softcap tanh(s / softcap) if softcap > 0;  s -= alibi_slopes[head] (p_t - x),
+ * the output sum e^s v / sum e^s, lse = ln sum e^s, and with mass  mass[r, h, i] += sum over tokens and the group's
+ * heads of e^s / sum e^s.  A token that sees no key has output 0 and lse -inf.  Keys that no token sees are not read:
+ * their slots may hold anything.  A block-table entry outside 0 .. num_blocks - 1 means "not in the cache": its keys
+ * are invisible.  n is clamped to 0 .. min(slot_capacity, max_blocks * block_size); n <= 0 is an idle request. */
+typedef struct pqhsa_paged_params {
+  int32_t abi_version;     /* PQHSA_ABI_VERSION */
+  int32_t dtype;           /* enum pqhsa_dtype of q, K/V and out */
+  int32_t requests;        /* B, 0 = nothing to do */
+  int32_t kv_heads;
+  int32_t group;           /* query heads per KV head, 1 .. 16 */
+  int32_t query_len;       /* T, 1 .. 8 query tokens per request; group * T <= 64 */
+  int32_t head_dim;        /* 128 */
+  int32_t slot_capacity;   /* row stride of key_pos and mass, most slots a request can hold (<= 2^24) */
+
+  const void *k_base, *v_base;   /* addressing as in pqhsa_params */
+  const int32_t *block_table;    /* [requests, max_blocks], or NULL: contiguous, block_size rows per request */
+  int32_t max_blocks, block_size, num_blocks;
+  int32_t window;          /* 0 = no window */
+  int64_t stride_block, stride_head, stride_row;
+
+  float scale, softcap;    /* softcap 0 = none */
+  const float *alibi_slopes;     /* [kv_heads * group] or NULL */
+  int32_t sink_tokens;     /* first positions that stay visible outside the window, and that an eviction keeps */
+  int32_t reserved;
+
+  const int32_t *seq_lens;       /* [requests] */
+  const int32_t *first_key;      /* [requests] or NULL */
+  const int32_t *query_pos;      /* [requests] position of the last query token; the attention requires it with key_pos */
+  int32_t *key_pos;              /* [requests, kv_heads, slot_capacity] or NULL: slots are positions */
+  float *mass;                   /* [requests, kv_heads, slot_capacity] or NULL */
+
+  const void *q;                 /* E; element strides from one request, token and query head to the next */
+  int64_t q_stride_request, q_stride_token, q_stride_head;
+  void *out;
+  int64_t out_stride_request, out_stride_token, out_stride_head;
+  float *lse;                    /* [requests, query_len, kv_heads * group] or NULL */
+  void *workspace;               /* >= pqhsa_paged_workspace_bytes(), 256-byte aligned, its first 4096 bytes zero before
+                                    the first use (the kernels leave them zero).  Calls that can overlap on the GPU need
+                                    one each */
+  size_t workspace_bytes;
+} pqhsa_paged_params;
+
+/* Workspace of pqhsa_paged_attention for these sizes (requests, heads, query_len, and slot_capacity if mass is set).
+ * A workspace made for a larger call serves a smaller one. */
+size_t pqhsa_paged_workspace_bytes(const pqhsa_paged_params* p);
+
+/* The attention above; the step's own K/V rows are in the pages already (counted in seq_lens). */
+int pqhsa_paged_attention(const pqhsa_paged_params* p, void* stream);
+
+/* Write new rows k, v (strides q_stride_* of p, over KV heads) of query_len tokens per request to slots
+ * seq_lens[r] .. + query_len - 1, their positions (the slots themselves without query_pos) to key_pos and 0 to mass (where given); new_lens[r] = seq_lens[r] +
+ * query_len (may be seq_lens itself).  A negative length is an idle request and stays; rows past the request's slots
+ * or on missing pages are dropped. */
+int pqhsa_paged_append(const pqhsa_paged_params* p, const void* k, const void* v, int32_t* new_lens, void* stream);
+
+/* Keep, per request and KV head, the `budget` slots of the largest mass - the sink_tokens first and the `recent` last
+ * positions (x > query_pos[r] - recent) before all others, NaN behind all, ties to the lower slot - in slots
+ * 0 .. budget - 1: a kept slot below the budget stays, the i-th of the other slots below it (ascending) takes over the
+ * i-th kept slot behind it: its K and V rows in place, its mass and position in new_mass / new_pos (may be mass /
+ * key_pos themselves).  source int32 [requests, kv_heads, budget] receives the slot each slot now holds (-1 past the
+ * request's keys), new_lens[r] = min(seq_lens[r], budget) (may be seq_lens itself).  holes: scratch like source.
+ * Slots behind the new length are left as they were.  Needs mass, key_pos and query_pos; the pages must belong to
+ * one request each. */
+int pqhsa_paged_evict(const pqhsa_paged_params* p, int32_t budget, int32_t recent, int32_t* new_lens, float* new_mass,
+                      int32_t* new_pos, int32_t* source, int32_t* holes, void* stream);
+
+/* 0 if `stream` is not being captured into a CUDA graph, else the capture's id: a host that keeps one workspace per
+ * stream of execution tells captures apart by it. */
+unsigned long long pqhsa_stream_capture_id(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,8 @@ _LAZY = {
     "IVFPQDecodeAttentionAdapter": "decode_adapter",
     "DecodeAttentionOutput": "decode_adapter",
     "GQASidecar": "gqa_sidecar",
+    "PagedAttention": "paged_attention",
+    "EvictingCacheAdapter": "evicting_cache",
 }
 
 __all__ = ["__version__", *_LAZY]

@@ -64,6 +64,26 @@ class WsLayout(C.Structure):
     ]
 
 
+class PagedParams(C.Structure):
+    """``pqhsa_paged_params`` of include/pqhsa.h, field for field."""
+
+    _fields_ = [
+        ("abi_version", C.c_int32), ("dtype", C.c_int32), ("requests", C.c_int32), ("kv_heads", C.c_int32),
+        ("group", C.c_int32), ("query_len", C.c_int32), ("head_dim", C.c_int32), ("slot_capacity", C.c_int32),
+        ("k_base", C.c_void_p), ("v_base", C.c_void_p), ("block_table", C.c_void_p),
+        ("max_blocks", C.c_int32), ("block_size", C.c_int32), ("num_blocks", C.c_int32), ("window", C.c_int32),
+        ("stride_block", C.c_int64), ("stride_head", C.c_int64), ("stride_row", C.c_int64),
+        ("scale", C.c_float), ("softcap", C.c_float), ("alibi_slopes", C.c_void_p),
+        ("sink_tokens", C.c_int32), ("reserved", C.c_int32),
+        ("seq_lens", C.c_void_p), ("first_key", C.c_void_p), ("query_pos", C.c_void_p), ("key_pos", C.c_void_p),
+        ("mass", C.c_void_p),
+        ("q", C.c_void_p), ("q_stride_request", C.c_int64), ("q_stride_token", C.c_int64), ("q_stride_head", C.c_int64),
+        ("out", C.c_void_p), ("out_stride_request", C.c_int64), ("out_stride_token", C.c_int64),
+        ("out_stride_head", C.c_int64),
+        ("lse", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 EXPORTS = {
     "pqhsa_abi_version": (C.c_int, []),
     "pqhsa_last_error_string": (C.c_char_p, []),
@@ -104,6 +124,14 @@ EXPORTS = {
         C.c_int,
         [C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p],
     ),
+    "pqhsa_paged_workspace_bytes": (C.c_size_t, [C.POINTER(PagedParams)]),
+    "pqhsa_paged_attention": (C.c_int, [C.POINTER(PagedParams), C.c_void_p]),
+    "pqhsa_paged_append": (C.c_int, [C.POINTER(PagedParams), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "pqhsa_paged_evict": (
+        C.c_int,
+        [C.POINTER(PagedParams), C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p],
+    ),
+    "pqhsa_stream_capture_id": (C.c_ulonglong, [C.c_void_p]),
 }
 
 

@@ -1,0 +1,175 @@
+// Shared parts of the dense paged-cache kernels (paged_attend.cu, paged_evict.cu): the argument block, which keys of
+// a request are visible, and how the key tiles of all requests are shared out over a persistent grid.
+#pragma once
+
+#include "common.cuh"
+
+namespace pqhsa {
+
+constexpr int kPagedGroupRows = 32;    // query rows of one KV head that go through the cache together
+constexpr int kPagedMaxRows = 64;      // query_len * group at most: two passes of kPagedGroupRows
+constexpr int kPagedMaxQuery = 8;
+constexpr int kPagedMaxCtas = 1024;    // counters in the workspace (one per CTA of the attention kernel)
+
+struct PagedArgs {
+  const void* k_base;
+  const void* v_base;
+  const int32_t* block_table;  // null: contiguous, request r is page r of block_size rows
+  int32_t max_blocks, block_size, num_blocks;
+  int64_t stride_block, stride_head, stride_row;
+  int32_t B, H, G, T, R;       // requests, KV heads, query heads per KV head, query tokens, R = G * T rows
+  int32_t groups;              // passes over a KV head's keys: ceil(R / kPagedGroupRows)
+  int32_t cap;                 // row stride of key_pos / mass / scores
+  int32_t limit;               // slots a request can have: min(cap, what its block-table row addresses)
+  float scale_log2, softcap, cap_log2, cap_in;  // see score() in paged_attend.cu
+  const float* slopes;
+  int32_t window, sinks;
+  const int32_t* seq_lens;
+  const int32_t* first_key;
+  const int32_t* query_pos;
+  const int32_t* key_pos;
+  float* mass;
+  const void* q;
+  int64_t q_sr, q_st, q_sh;
+  void* out;
+  int64_t o_sr, o_st, o_sh;
+  float* lse;
+  int32_t* tickets;            // [kPagedMaxCtas], zero between launches
+  float2* part_ml;             // [2 * CTAs][kPagedGroupRows] (max, sum) of a stream's part
+  float* part_acc;             // [2 * CTAs][rows of a pass][128]
+  float* row_lse2;             // [B * H][R] log2 sum 2^s of every query row
+  float* scores;               // [B * H][R][cap] scores in log2 units, only with mass
+  int32_t tile_log2;           // keys per tile of the attention kernel that runs (fixes the shares)
+};
+
+int launch_paged_attend(const PagedArgs& a, int dtype, cudaStream_t st);
+int launch_paged_mass(const PagedArgs& a, cudaStream_t st);
+
+struct PagedEvict {
+  int32_t budget, recent;
+  int32_t* new_lens;   // may be the lengths read
+  float* new_mass;     // [B, H, cap], may be the mass read
+  int32_t* new_pos;    // [B, H, cap], may be the positions read
+  int32_t* source;     // [B, H, budget]
+  int32_t* holes;      // workspace [B, H, budget]
+};
+int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaStream_t st);
+int launch_paged_append(const PagedArgs& a, const void* k, const void* v, int32_t* new_lens, int dtype, cudaStream_t st);
+
+#ifdef __CUDACC__
+
+// Element offset of slot t of request r, KV head h; negative when the slot's page is not in the cache (a block-table
+// entry outside 0 .. num_blocks - 1: such a key is invisible, nothing of it is read or written).
+__device__ __forceinline__ int64_t paged_offset(const PagedArgs& a, int r, int h, int t) {
+  int64_t blk = r;
+  int row = t;
+  if (a.block_table != nullptr) {
+    const int b = t / a.block_size;
+    row = t - b * a.block_size;
+    const int32_t e = __ldg(a.block_table + (int64_t)r * a.max_blocks + b);
+    if (e < 0 || e >= a.num_blocks) return -1;
+    blk = e;
+  }
+  return blk * a.stride_block + (int64_t)h * a.stride_head + (int64_t)row * a.stride_row;
+}
+
+// What a request's query tokens can see.  Query token t sits at position p_first + t; a key at position x is visible
+// to position p when first <= x <= p and (no window, or p - x < window, or x - first < sinks).  Slots are positions
+// unless key_pos says otherwise; then every slot has to be looked at, else only the tiles of [first, first + sinks)
+// and of the window.
+struct PagedGeom {
+  int n, first, p_first, p_last;
+  int a0, na, b0, tiles;  // tiles a0 .. a0 + na, then b0 ..; tiles >= 1, so that every row gets its output
+};
+__device__ __forceinline__ PagedGeom paged_geom(const PagedArgs& a, int r) {
+  PagedGeom g;
+  g.n = min(max(__ldg(a.seq_lens + r), 0), a.limit);
+  g.first = a.first_key != nullptr ? max(__ldg(a.first_key + r), 0) : 0;
+  g.p_last = a.query_pos != nullptr ? max(__ldg(a.query_pos + r), -1) : g.n - 1;
+  g.p_first = g.p_last - (a.T - 1);
+  const int tl = a.tile_log2, up = (1 << tl) - 1;
+  const int end = (g.n + up) >> tl;
+  g.a0 = g.na = g.b0 = 0;
+  if (a.key_pos == nullptr) {
+    const int lo = min(g.first, g.n);
+    g.b0 = lo >> tl;
+    if (a.window > 0) {
+      const int w = min(max(lo, g.p_first - a.window + 1), g.n);       // first slot of the window
+      const int s = min(a.sinks, w - lo);                              // sink slots in front of it
+      g.a0 = lo >> tl;
+      g.na = s > 0 ? ((lo + s + up) >> tl) - g.a0 : 0;
+      g.b0 = max(w >> tl, g.a0 + g.na);
+    }
+  }
+  g.tiles = max(g.na + max(end - g.b0, 0), 1);
+  return g;
+}
+__device__ __forceinline__ int paged_tile(const PagedGeom& g, int j) { return j < g.na ? g.a0 + j : g.b0 + j - g.na; }
+__device__ __forceinline__ bool paged_sees(const PagedGeom& g, const PagedArgs& a, int x, int p) {
+  return x >= g.first && x <= p && (a.window == 0 || p - x < a.window || x - g.first < a.sinks);
+}
+
+// The tiles of all streams - stream (r, h, pass) in that order - form one sequence, of which CTA c takes the share
+// [total c / C, total (c + 1) / C): equal shares whatever the lengths.  Every warp finds its CTA's share by itself.
+__device__ __forceinline__ long long paged_share(long long total, int c, int C) { return total * c / C; }
+
+struct PagedCursor {
+  int r, sub;       // request; pass + groups * KV head
+  int tile;         // next tile of that stream
+  PagedGeom g;
+};
+
+// Sum of the requests' tiles times the streams per request (all lanes call).
+__device__ __forceinline__ long long paged_total(const PagedArgs& a) {
+  const int lane = threadIdx.x & 31;
+  long long sum = 0;
+  for (int r = lane; r < a.B; r += 32) sum += paged_geom(a, r).tiles;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum * (a.H * a.groups);
+}
+
+// Cursor at place x of the sequence (x < total; all lanes call).
+__device__ __forceinline__ PagedCursor paged_locate(const PagedArgs& a, long long x) {
+  const int lane = threadIdx.x & 31, per = a.H * a.groups;
+  PagedCursor c;
+  long long before = 0;
+  int base = 0;
+  while (true) {
+    const int r = base + lane;
+    const long long mine = r < a.B ? (long long)paged_geom(a, r).tiles * per : 0;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, before + incl > x);
+    if (past != 0u || base + 32 >= a.B) {
+      const int at = past != 0u ? __ffs(past) - 1 : 31;
+      c.r = min(base + at, a.B - 1);
+      before += __shfl_sync(0xffffffffu, incl - mine, at);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+    base += 32;
+  }
+  c.g = paged_geom(a, c.r);
+  const int inside = (int)(x - before);  // the host refuses shapes whose tiles of one request pass 31 bits
+  c.sub = inside / c.g.tiles;
+  c.tile = inside - c.sub * c.g.tiles;
+  return c;
+}
+
+__device__ __forceinline__ void paged_next_stream(const PagedArgs& a, PagedCursor& c) {
+  c.tile = 0;
+  if (++c.sub == a.H * a.groups) {
+    c.sub = 0;
+    ++c.r;
+    if (c.r < a.B) c.g = paged_geom(a, c.r);
+  }
+}
+
+#endif  // __CUDACC__
+
+}  // namespace pqhsa
