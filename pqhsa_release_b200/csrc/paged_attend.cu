@@ -356,6 +356,369 @@ static int launch_simple(const PagedArgs& a, cudaStream_t st) {
   return check_launch("paged_attend");
 }
 
+// ---- tensor-core kernel for 16-bit caches: tiles of 16 keys ----------------------------------------------
+// Both products run transposed, so that the many keys (and dimensions) are the 16 rows of an m16n8k16 and the few query
+// rows its 8 columns: S^T[16 keys, 8 rows] = K q^T and O^T[16 dims, 8 rows] += V^T P^T.  K rows are the A operand as they
+// lie (ldmatrix), V the A operand transposed (ldmatrix.trans); P^T gets from the accumulator layout of S^T into the B
+// layout with one 8x8 transpose in registers per 8 keys.  A thread holds the same two query rows of every 8 in S^T and
+// in O^T, so maxima, sums and rescaling need no exchange.  p is rounded to the 16-bit type for the product with V (half
+// a step of a value in 0 .. 2^8; the sum it is divided by keeps 32 bits).  Against one row per m16 (P V with 16 rows
+// of which 4 or 8 are real) this halves the instructions and the accumulators.
+constexpr int kMKeys = 16;
+
+template <typename E> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t smem) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t smem) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <typename E> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A warp's view of the tiles it has still to fetch: lane i < 16 looks after key i.  What the addresses depend on (page
+// table, stored positions) is requested one tile before it is needed.
+struct TileFetch {
+  int32_t entry;  // page
+  int32_t row;    // row in the page
+  int32_t pos;    // position, or a value no token sees
+};
+
+template <typename E, int NB, int STAGES>
+__global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const PagedArgs a) {
+  constexpr int ROWS = 8 * NB;
+  constexpr bool QREG = NB <= 2;  // query rows as B fragments in registers; from shared memory when they would fill them
+  constexpr int kStageB = 2 * kMKeys * kD * 2;  // bytes of a stage: 16 key rows, then 16 value rows, 256 bytes each
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  constexpr size_t kRing = (size_t)kPWarps * STAGES * kStageB;
+  constexpr size_t kMerge = sizeof(float) * kPWarps * ROWS * kAccStride;
+  float* acc_s = reinterpret_cast<float*>(smem_raw);  // merge buffer over the rings, used between streams
+  uint8_t* tail = smem_raw + (kRing > kMerge ? kRing : kMerge);
+  float2* ml_s = reinterpret_cast<float2*>(tail);                 // [warps][ROWS]
+  uint8_t* q_s = tail + sizeof(float2) * kPWarps * ROWS;          // [ROWS][128] E, pieces swizzled, only without QREG
+  __shared__ int pos_s[kPWarps][STAGES][kMKeys];
+  __shared__ int seen_s[kPWarps][STAGES];   // keys some row of the step sees; << 16: keys not all of them see
+  __shared__ int last_s;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t4 = lane & 3, l4 = lane >> 2;
+  const E* kb = static_cast<const E*>(a.k_base);
+  const E* vb = static_cast<const E*>(a.v_base);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem_raw) + warp * (STAGES * kStageB);
+  // shared-memory addresses inside a tile, before the 16-byte piece is added: piece j of row k lies at j ^ (k & 7)
+  const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_hi = lane >> 4;          // K: rows 0-7 | 8-15, then the upper 8 dims
+  const int v_row = (lane & 7) + (lane >> 4) * 8, v_hi = (lane >> 3) & 1;          // V: upper 8 dims, then rows 8-15
+  const int g_row = lane >> 3, g_piece = lane & 7;                                 // copies: 4 rows x 128 bytes at a time
+
+  const long long total = paged_total(a);
+  const int C = (int)min((long long)gridDim.x, total);  // CTAs with a share: none of them is empty
+  if (blockIdx.x >= C) return;
+  long long x = paged_share(total, blockIdx.x, C);
+  const long long x_end = paged_share(total, blockIdx.x + 1, C);
+  PagedCursor c = paged_locate(a, x);
+
+  while (true) {
+    const int count = (int)min((long long)(c.g.tiles - c.tile), x_end - x);  // tiles of this stream in the share
+    const int pass = c.sub % a.groups, h = c.sub / a.groups;
+    const int row0 = pass * kPagedGroupRows, rows = min(a.R - row0, kPagedGroupRows);
+    const int mine = count > warp ? (count - warp + kPWarps - 1) / kPWarps : 0;
+    const int32_t* kpos = a.key_pos != nullptr ? a.key_pos + ((int64_t)c.r * a.H + h) * a.cap : nullptr;
+    const int32_t* table = a.block_table != nullptr ? a.block_table + (int64_t)c.r * a.max_blocks : nullptr;
+
+    auto fetch = [&](int it) {
+      TileFetch f = {-1, 0, -1};
+      if (it < mine && lane < kMKeys) {
+        const int slot = paged_tile(c.g, c.tile + warp + it * kPWarps) * kMKeys + lane;
+        if (slot < c.g.n) {
+          f.pos = kpos != nullptr ? __ldg(kpos + slot) : slot;
+          f.entry = c.r;
+          f.row = slot;
+          if (table != nullptr) {
+            const int b = slot / a.block_size;
+            f.row = slot - b * a.block_size;
+            f.entry = __ldg(table + b);
+          }
+        }
+      }
+      return f;
+    };
+    auto load = [&](int it, int st, const TileFetch& f) {
+      if (it < mine) {
+        bool any = f.entry >= 0 && f.entry < a.num_blocks && f.pos >= c.g.first && f.pos <= c.g.p_last;
+        bool all = f.pos <= c.g.p_first;
+        if (a.window > 0) {
+          const bool sink = f.pos - c.g.first < a.sinks;
+          any = any && (c.g.p_first - f.pos < a.window || sink);
+          all = all && (c.g.p_last - f.pos < a.window || sink);
+        }
+        const unsigned seen = __ballot_sync(0xffffffffu, any), mixed = __ballot_sync(0xffffffffu, any && !all);
+        if (lane < kMKeys) pos_s[warp][st][lane] = f.pos;
+        if (lane == 0) seen_s[warp][st] = (int)((seen & 0xffffu) | (mixed << 16));
+        const int64_t off = any ? f.entry * a.stride_block + h * a.stride_head + f.row * a.stride_row : 0;
+        const uint32_t dst = ring + st * kStageB;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = 4 * i + g_row;
+          const int64_t o = __shfl_sync(0xffffffffu, off, k) + g_piece * 8;
+          const bool take = (seen >> k) & 1u;
+          const uint32_t to = dst + k * 256 + ((g_piece ^ (k & 7)) << 4);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            cp_async16_zfill(to + j * 128, kb + o + j * 64, take);
+            cp_async16_zfill(to + j * 128 + kMKeys * 256, vb + o + j * 64, take);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+
+    uint32_t qf[QREG ? NB : 1][8][2];
+    if constexpr (!QREG) __syncthreads();  // q_s of the stream before has been read
+    if constexpr (QREG) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const int row = 8 * nb + l4, full = row0 + row;
+        const E* src = static_cast<const E*>(a.q) + (int64_t)c.r * a.q_sr + (int64_t)(full / a.G) * a.q_st +
+                       (int64_t)(h * a.G + full % a.G) * a.q_sh + 2 * t4;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          qf[nb][kk][0] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
+          qf[nb][kk][1] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
+        }
+      }
+    } else {
+      for (int i = tid; i < ROWS * 16; i += kPThreads) {
+        const int row = i >> 4, piece = i & 15, full = row0 + row;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows)
+          v = __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + (int64_t)c.r * a.q_sr +
+                                                   (int64_t)(full / a.G) * a.q_st + (int64_t)(h * a.G + full % a.G) * a.q_sh) + piece);
+        *reinterpret_cast<uint4*>(q_s + row * 256 + ((piece ^ (row & 7)) << 4)) = v;
+      }
+      __syncthreads();
+    }
+    TileFetch next = fetch(0);
+#pragma unroll
+    for (int st = 0; st < STAGES - 1; ++st) {
+      const TileFetch f = next;
+      next = fetch(st + 1);
+      load(st, st, f);
+    }
+    float m[NB][2], l[NB][2], slope[NB][2], o[NB][8][4];
+    int p_at[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = 8 * nb + 2 * t4 + j, full = row0 + row;
+        m[nb][j] = kNegInf;
+        l[nb][j] = 0.f;
+        p_at[nb][j] = row < rows ? c.g.p_first + full / a.G : -1;
+        slope[nb][j] = row < rows && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + full % a.G) : 0.f;
+      }
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[nb][db][j] = 0.f;
+    }
+
+    for (int it = 0; it < mine; ++it) {
+      const int st = it % STAGES;
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();
+      {
+        const TileFetch f = next;
+        next = fetch(it + STAGES);
+        load(it + STAGES - 1, (it + STAGES - 1) % STAGES, f);
+      }
+      const uint32_t kt = ring + st * kStageB, vt = kt + kMKeys * 256;
+      float s[NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[nb][j] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < 8; kk += 2) {
+        uint32_t a0[4], a1[4];
+        ldmatrix4(a0, kt + k_row * 256 + (((2 * kk + k_hi) ^ (k_row & 7)) << 4));
+        ldmatrix4(a1, kt + k_row * 256 + (((2 * kk + 2 + k_hi) ^ (k_row & 7)) << 4));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          if constexpr (QREG) {
+            mma16816<E>(s[nb], a0, qf[nb][kk][0], qf[nb][kk][1]);
+            mma16816<E>(s[nb], a1, qf[nb][kk + 1][0], qf[nb][kk + 1][1]);
+          } else {
+            uint32_t b[4];
+            const int row = 8 * nb + (lane & 7), piece = 2 * kk + (lane >> 3);
+            ldmatrix4(b, (uint32_t)__cvta_generic_to_shared(q_s) + row * 256 + ((piece ^ (row & 7)) << 4));
+            mma16816<E>(s[nb], a0, b[0], b[1]);
+            mma16816<E>(s[nb], a1, b[2], b[3]);
+          }
+        }
+      }
+      // s[nb][0], [1]: key l4, rows 2 t4 and 2 t4 + 1 of block nb; [2], [3]: key l4 + 8
+      const unsigned flags = (unsigned)seen_s[warp][st];
+      const int pos0 = pos_s[warp][st][l4], pos1 = pos_s[warp][st][l4 + 8];
+      const bool seen0 = (flags >> l4) & 1u, seen1 = (flags >> (l4 + 8)) & 1u;
+      const unsigned mixed = flags >> 16;
+      bool raise = false;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int pos = j < 2 ? pos0 : pos1, p = p_at[nb][j & 1];
+          bool vis = (j < 2 ? seen0 : seen1) && p >= 0;
+          if (mixed != 0u) vis = vis && paged_sees(c.g, a, pos, p);
+          s[nb][j] = vis ? paged_score(a, s[nb][j], slope[nb][j & 1], p - pos) : kNegInf;
+          raise |= s[nb][j] > m[nb][j & 1] + kLazy;
+        }
+      }
+      if (a.scores != nullptr) {
+        const int slot = paged_tile(c.g, c.tile + warp + it * kPWarps) * kMKeys + l4;
+        float* dst = a.scores + (((int64_t)c.r * a.H + h) * a.R + row0 + 2 * t4) * a.cap + slot;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (8 * nb + 2 * t4 + (j & 1) < rows && slot + (j >> 1) * 8 < c.g.n)
+              dst[(int64_t)(8 * nb + (j & 1)) * a.cap + (j >> 1) * 8] = s[nb][j];
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = fmaxf(s[nb][j], s[nb][j + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float to = fmaxf(m[nb][j], top);
+            const float f = m[nb][j] == kNegInf ? (to == kNegInf ? 1.f : 0.f) : ex2(m[nb][j] - to);
+            m[nb][j] = to;
+            l[nb][j] *= f;
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+              o[nb][db][j] *= f;
+              o[nb][db][j + 2] *= f;
+            }
+          }
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[nb][j] = s[nb][j] == kNegInf ? 0.f : ex2(s[nb][j] - m[nb][j & 1]);
+          l[nb][j & 1] += s[nb][j];
+        }
+      if (mixed != 0u) {
+        // Keys that only some rows see (at most the last query_len - 1 and as many at the window's edge): a product with
+        // p = 0 would let an infinite or NaN value through, so these are added one by one and then taken out.
+        uint8_t* vrow = smem_raw + (vt - (uint32_t)__cvta_generic_to_shared(smem_raw));
+        unsigned left = mixed;
+        while (left != 0u) {
+          const int k = __ffs(left) - 1;
+          left &= left - 1;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const float pa = __shfl_sync(0xffffffffu, k < 8 ? s[nb][0] : s[nb][2], (k & 7) * 4 + t4);
+            const float pb = __shfl_sync(0xffffffffu, k < 8 ? s[nb][1] : s[nb][3], (k & 7) * 4 + t4);
+#pragma unroll
+            for (int d = 0; d < 16; ++d) {
+              const float v = to_f(*reinterpret_cast<const E*>(vrow + k * 256 + ((d ^ (k & 7)) << 4) + l4 * 2));
+              float& oa = o[nb][d >> 1][(d & 1) * 2];
+              float& ob = o[nb][d >> 1][(d & 1) * 2 + 1];
+              oa = pa != 0.f ? fmaf(pa, v, oa) : oa;
+              ob = pb != 0.f ? fmaf(pb, v, ob) : ob;
+            }
+          }
+          __syncwarp();
+          *reinterpret_cast<uint2*>(vrow + k * 256 + lane * 8) = make_uint2(0u, 0u);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          if ((mixed >> l4) & 1u) s[nb][0] = s[nb][1] = 0.f;
+          if ((mixed >> (l4 + 8)) & 1u) s[nb][2] = s[nb][3] = 0.f;
+        }
+      }
+      uint32_t pf[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        pf[nb][0] = transpose8x8(pack2<E>(s[nb][0], s[nb][1]));
+        pf[nb][1] = transpose8x8(pack2<E>(s[nb][2], s[nb][3]));
+      }
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        uint32_t av[4];
+        ldmatrix4_trans(av, vt + v_row * 256 + (((2 * db + v_hi) ^ (v_row & 7)) << 4));
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma16816<E>(o[nb][db], av, pf[nb][0], pf[nb][1]);
+      }
+      __syncwarp();  // the slot may be filled again
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // every warp is done with its ring: the merge buffer lies over it
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], d);
+        if (l4 == 0) ml_s[warp * ROWS + 8 * nb + 2 * t4 + j] = make_float2(m[nb][j], l[nb][j]);
+      }
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc_s[((size_t)warp * ROWS + 8 * nb + 2 * t4 + (j & 1)) * kAccStride + db * 16 + l4 + (j >> 1) * 8] = o[nb][db][j];
+    }
+    __syncthreads();
+    paged_finish<E>(a, c, x - c.tile, c.tile, count, total, C, rows, ROWS, ml_s, acc_s, &last_s);
+    x += count;
+    if (x >= x_end) return;
+    __syncthreads();  // the rings are free again
+    paged_next_stream(a, c);
+  }
+}
+
+template <typename E, int NB, int STAGES>
+static int launch_mma(const PagedArgs& a, cudaStream_t st) {
+  constexpr int ROWS = 8 * NB;
+  constexpr size_t ring = (size_t)kPWarps * STAGES * 2 * kMKeys * kD * 2;
+  constexpr size_t merge = sizeof(float) * kPWarps * ROWS * kAccStride;
+  constexpr size_t smem = (ring > merge ? ring : merge) + sizeof(float2) * kPWarps * ROWS + (NB > 2 ? ROWS * 256 : 0);
+  static_assert(smem <= 220 * 1024, "shared memory of a CTA");
+  auto kern = paged_attend_mma_kernel<E, NB, STAGES>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return check_launch("paged_attend shared memory");
+  kern<<<sm_count(), kPThreads, smem, st>>>(a);
+  return check_launch("paged_attend");
+}
+
 // ---- accumulated weights -----------------------------------------------------------------------------
 // mass[r, h, i] += sum over the rows of 2^(s - lse): one pass over the scores the attention kernel left (4 bytes per
 // row and key, which come from L2 while the cache rows went past it), the same shares of the same tiles.  The rows of
@@ -396,12 +759,21 @@ int launch_paged_mass(const PagedArgs& a, cudaStream_t st) {
 
 int launch_paged_attend(const PagedArgs& a, int dtype, cudaStream_t st) {
   PagedArgs b = a;
-  b.tile_log2 = 3;
-  int rc = PQHSA_OK;
   const int rows = a.R < kPagedGroupRows ? a.R : kPagedGroupRows;
-  PQHSA_DISPATCH_E(dtype, {
-    rc = rows <= 8 ? launch_simple<E, 8, 2>(b, st) : rows <= 16 ? launch_simple<E, 16, 2>(b, st) : launch_simple<E, 32, 2>(b, st);
-  });
+  int rc = PQHSA_OK;
+  if (dtype == PQHSA_F32) {
+    b.tile_log2 = 3;
+    rc = rows <= 8 ? launch_simple<float, 8, 2>(b, st) : rows <= 16 ? launch_simple<float, 16, 2>(b, st) : launch_simple<float, 32, 2>(b, st);
+  } else {
+    b.tile_log2 = 4;
+    if (dtype == PQHSA_BF16) {
+      using E = __nv_bfloat16;
+      rc = rows <= 8 ? launch_mma<E, 1, 3>(b, st) : rows <= 16 ? launch_mma<E, 2, 3>(b, st) : launch_mma<E, 4, 3>(b, st);
+    } else {
+      using E = __half;
+      rc = rows <= 8 ? launch_mma<E, 1, 3>(b, st) : rows <= 16 ? launch_mma<E, 2, 3>(b, st) : launch_mma<E, 4, 3>(b, st);
+    }
+  }
   if (rc != PQHSA_OK || a.mass == nullptr) return rc;
   return launch_paged_mass(b, st);
 }
