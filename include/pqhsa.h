@@ -480,11 +480,11 @@ int pqhsa_paged_append(const pqhsa_paged_params* p, const void* k, const void* v
  * 0 .. budget - 1: a kept slot below the budget stays, the i-th of the other slots below it (ascending) takes over the
  * i-th kept slot behind it: its K and V rows in place, its mass and position in new_mass / new_pos (may be mass /
  * key_pos themselves).  source int32 [requests, kv_heads, budget] receives the slot each slot now holds (-1 past the
- * request's keys), new_lens[r] = min(seq_lens[r], budget) (may be seq_lens itself).  holes: scratch like source.
- * Slots behind the new length are left as they were.  Needs mass, key_pos and query_pos; the pages must belong to
- * one request each. */
+ * request's keys), new_lens[r] = min(seq_lens[r], budget) (may be seq_lens itself).  scratch: int32 [requests,
+ * kv_heads, 2 * budget + 8].  requests * kv_heads <= 65535.  Slots behind the new length are left as they were.
+ * Needs mass, key_pos and query_pos; the pages must belong to one request each. */
 int pqhsa_paged_evict(const pqhsa_paged_params* p, int32_t budget, int32_t recent, int32_t* new_lens, float* new_mass,
-                      int32_t* new_pos, int32_t* source, int32_t* holes, void* stream);
+                      int32_t* new_pos, int32_t* source, int32_t* scratch, void* stream);
 
 /* 0 if `stream` is not being captured into a CUDA graph, else the capture's id: a host that keeps one workspace per
  * stream of execution tells captures apart by it. */

@@ -51,12 +51,16 @@ struct PagedEvict {
   float* new_mass;     // [B, H, cap], may be the mass read
   int32_t* new_pos;    // [B, H, cap], may be the positions read
   int32_t* source;     // [B, H, budget]
-  int32_t* holes;      // workspace [B, H, budget]
+  int32_t* scratch;    // [B, H, 2 budget + 8]: moves, then (from 8) the slots to fill and (from 8 + budget) those that fill them
 };
 int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaStream_t st);
 int launch_paged_append(const PagedArgs& a, const void* k, const void* v, int32_t* new_lens, int dtype, cudaStream_t st);
 
 #ifdef __CUDACC__
+
+// A kernel launched with programmatic stream serialization starts while the one before it ends; from here on it sees
+// all that one wrote.
+__device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Element offset of slot t of request r, KV head h; negative when the slot's page is not in the cache (a block-table
 // entry outside 0 .. num_blocks - 1: such a key is invisible, nothing of it is read or written).

@@ -142,16 +142,17 @@ int pqhsa_paged_append(const pqhsa_paged_params* p, const void* k, const void* v
 }
 
 int pqhsa_paged_evict(const pqhsa_paged_params* p, int32_t budget, int32_t recent, int32_t* new_lens, float* new_mass,
-                      int32_t* new_pos, int32_t* source, int32_t* holes, void* stream) {
+                      int32_t* new_pos, int32_t* source, int32_t* scratch, void* stream) {
   if (int rc = check_paged(p)) return rc;
   if (p->requests == 0) return PQHSA_OK;
   if (int rc = check_cache(p)) return rc;
   if (!p->mass || !p->key_pos || !p->query_pos) return set_error(PQHSA_E_NULL, "an eviction needs mass, key_pos and query_pos");
-  if (!new_lens || !new_mass || !new_pos || !source || !holes) return set_error(PQHSA_E_NULL, "an output of the eviction is null");
+  if (!new_lens || !new_mass || !new_pos || !source || !scratch) return set_error(PQHSA_E_NULL, "an output of the eviction is null");
   if (budget < 1 || budget > (1 << 24)) return set_error(PQHSA_E_SHAPE, "budget must be in 1..2^24, got %d", budget);
   if (recent < 0 || (long long)recent + p->sink_tokens > budget)
     return set_error(PQHSA_E_SHAPE, "sink_tokens %d + recent %d must fit the budget %d", p->sink_tokens, recent, budget);
-  const PagedEvict e = {budget, recent, new_lens, new_mass, new_pos, source, holes};
+  if ((long long)p->requests * p->kv_heads > 65535) return set_error(PQHSA_E_SHAPE, "requests * kv_heads must be at most 65535");
+  const PagedEvict e = {budget, recent, new_lens, new_mass, new_pos, source, scratch};
   return launch_paged_evict(paged_args(p), e, p->dtype, (cudaStream_t)stream);
 }
 

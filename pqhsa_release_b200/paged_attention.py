@@ -299,14 +299,14 @@ class PagedAttention:
         nm = p.mass if new_mass is None else self._per_slot(new_mass, "new_mass", torch.float32, B)
         npos = p.key_pos if new_pos is None else self._per_slot(new_pos, "new_pos", torch.int32, B)
         with torch.cuda.device(self._index):
-            n = 4 * B * self.H * budget
-            holes, stream = self._scratch("evict", 2 * n)
+            n = 4 * B * self.H * (2 * budget + 8)
+            scratch, stream = self._scratch("evict", n + 4 * B * self.H * budget)
             if source is None:
-                src = holes + n
+                src = scratch + n
             else:
                 if (source.dtype is not torch.int32 or source.device != self.device or tuple(source.shape) != (B, self.H, budget)
                         or not source.is_contiguous()):
                     raise ValueError(f"source must be a contiguous int32 [{B}, {self.H}, {budget}] tensor on {self.device}")
                 src = source.data_ptr()
-            _lib.call("pqhsa_paged_evict", self._ref, budget, recent, to, nm, npos, src, holes, stream)
+            _lib.call("pqhsa_paged_evict", self._ref, budget, recent, to, nm, npos, src, scratch, stream)
         return new_lens
