@@ -38,7 +38,8 @@ struct PagedArgs {
   float2* part_ml;             // [2 * CTAs][kPagedGroupRows] (max, sum) of a stream's part
   float* part_acc;             // [2 * CTAs][rows of a pass][128]
   float* row_lse2;             // [B * H][R] log2 sum 2^s of every query row
-  float* scores;               // [B * H][R][cap] scores in log2 units, only with mass
+  float* scores;               // [B * H][R][score_stride] scores in log2 units, only with mass
+  int64_t score_stride;        // cap, rounded up to whole tiles
   int32_t tile_log2;           // keys per tile of the attention kernel that runs (fixes the shares)
 };
 
@@ -113,65 +114,92 @@ __device__ __forceinline__ bool paged_sees(const PagedGeom& g, const PagedArgs& 
   return x >= g.first && x <= p && (a.window == 0 || p - x < a.window || x - g.first < a.sinks);
 }
 
-// The tiles of all streams - stream (r, h, pass) in that order - form one sequence, of which CTA c takes the share
-// [total c / C, total (c + 1) / C): equal shares whatever the lengths.  Every warp finds its CTA's share by itself.
-__device__ __forceinline__ long long paged_share(long long total, int c, int C) { return total * c / C; }
+// Of a key at position x: whether some query token sees it, and whether all do (if some do).
+struct PagedSight {
+  bool any, all;
+};
+__device__ __forceinline__ PagedSight paged_sight(const PagedGeom& g, const PagedArgs& a, bool there, int x) {
+  PagedSight s;
+  s.any = there && x >= g.first && x <= g.p_last;
+  s.all = x <= g.p_first;
+  if (a.window > 0) {
+    const bool sink = x - g.first < a.sinks;
+    s.any = s.any && (g.p_first - x < a.window || sink);
+    s.all = s.all && (g.p_last - x < a.window || sink);
+  }
+  return s;
+}
+
+// The tiles of all streams - stream (r, h, pass) in that order - form one sequence of `total` (the host refuses shapes
+// that could pass 31 bits), of which each of C CTAs takes a contiguous share: total / C tiles, one more for the first
+// total % C of them.  Equal shares whatever the lengths; every warp finds its CTA's by itself.
+struct PagedShares {
+  int total, C, q, rem;
+  __device__ __forceinline__ int first(int c) const { return c * q + min(c, rem); }
+  __device__ __forceinline__ int owner(int x) const {  // CTA that has tile x
+    const int wide = rem * (q + 1);
+    return x < wide ? x / (q + 1) : rem + (x - wide) / q;
+  }
+};
+__device__ __forceinline__ PagedShares paged_shares(int total, int ctas) {
+  PagedShares s;
+  s.total = total;
+  s.C = min(ctas, total);  // CTAs with a share: none of them is empty
+  s.q = total / s.C;
+  s.rem = total - s.q * s.C;
+  return s;
+}
 
 struct PagedCursor {
-  int r, sub;       // request; pass + groups * KV head
+  int r, h, pass;   // request, KV head, pass over its keys
   int tile;         // next tile of that stream
   PagedGeom g;
 };
 
-// Sum of the requests' tiles times the streams per request (all lanes call).
-__device__ __forceinline__ long long paged_total(const PagedArgs& a) {
-  const int lane = threadIdx.x & 31;
-  long long sum = 0;
-  for (int r = lane; r < a.B; r += 32) sum += paged_geom(a, r).tiles;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum * (a.H * a.groups);
-}
-
-// Cursor at place x of the sequence (x < total; all lanes call).
-__device__ __forceinline__ PagedCursor paged_locate(const PagedArgs& a, long long x) {
+// Shares of this launch, and the cursor at the first tile of share c (c < shares.C, else the cursor is not set).  All
+// lanes of a warp call; lane l looks after requests l, l + 32, ...
+__device__ __forceinline__ PagedShares paged_locate(const PagedArgs& a, int ctas, int cta, PagedCursor& c) {
   const int lane = threadIdx.x & 31, per = a.H * a.groups;
-  PagedCursor c;
-  long long before = 0;
-  int base = 0;
-  while (true) {
-    const int r = base + lane;
-    const long long mine = r < a.B ? (long long)paged_geom(a, r).tiles * per : 0;
-    long long incl = mine;
+  int mine = lane < a.B ? paged_geom(a, lane).tiles : 0;
+  int sum = mine;
+  for (int r = lane + 32; r < a.B; r += 32) sum += paged_geom(a, r).tiles;
+  const PagedShares sh = paged_shares(__reduce_add_sync(0xffffffffu, sum) * per, ctas);
+  if (cta >= sh.C) return sh;
+  const int x = sh.first(cta);
+  int before = 0;
+  for (int base = 0;; base += 32) {
+    if (base > 0) mine = base + lane < a.B ? paged_geom(a, base + lane).tiles : 0;
+    int incl = mine * per;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, incl, o);
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
     const unsigned past = __ballot_sync(0xffffffffu, before + incl > x);
     if (past != 0u || base + 32 >= a.B) {
       const int at = past != 0u ? __ffs(past) - 1 : 31;
       c.r = min(base + at, a.B - 1);
-      before += __shfl_sync(0xffffffffu, incl - mine, at);
+      before += __shfl_sync(0xffffffffu, incl - mine * per, at);
       break;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);
-    base += 32;
   }
   c.g = paged_geom(a, c.r);
-  const int inside = (int)(x - before);  // the host refuses shapes whose tiles of one request pass 31 bits
-  c.sub = inside / c.g.tiles;
-  c.tile = inside - c.sub * c.g.tiles;
-  return c;
+  const int sub = (x - before) / c.g.tiles;
+  c.tile = x - before - sub * c.g.tiles;
+  c.h = sub / a.groups;
+  c.pass = sub - c.h * a.groups;
+  return sh;
 }
 
 __device__ __forceinline__ void paged_next_stream(const PagedArgs& a, PagedCursor& c) {
   c.tile = 0;
-  if (++c.sub == a.H * a.groups) {
-    c.sub = 0;
-    ++c.r;
-    if (c.r < a.B) c.g = paged_geom(a, c.r);
-  }
+  if (++c.pass < a.groups) return;
+  c.pass = 0;
+  if (++c.h < a.H) return;
+  c.h = 0;
+  ++c.r;
+  if (c.r < a.B) c.g = paged_geom(a, c.r);
 }
 
 #endif  // __CUDACC__

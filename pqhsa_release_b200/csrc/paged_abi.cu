@@ -7,6 +7,8 @@ namespace pqhsa {
 
 static inline size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
+static inline size_t paged_score_stride(int cap) { return ((size_t)cap + 15) / 16 * 16; }
+
 struct PagedWs {
   size_t part_ml, part_acc, row_lse2, scores, total;
 };
@@ -23,7 +25,7 @@ static PagedWs paged_ws(const pqhsa_paged_params* p) {
   w.row_lse2 = off;
   off = align256(off + streams * R * sizeof(float));
   w.scores = off;
-  if (p->mass != nullptr) off = align256(off + streams * R * (size_t)p->slot_capacity * sizeof(float));
+  if (p->mass != nullptr) off = align256(off + streams * R * paged_score_stride(p->slot_capacity) * sizeof(float));
   w.total = off;
   return w;
 }
@@ -43,8 +45,8 @@ static int check_paged(const pqhsa_paged_params* p) {
     return set_error(PQHSA_E_SHAPE, "group * query_len must be at most %d, got %d", kPagedMaxRows, p->group * p->query_len);
   if (p->slot_capacity < 1 || p->slot_capacity > (1 << 24))
     return set_error(PQHSA_E_SHAPE, "slot_capacity must be in 1..2^24, got %d", p->slot_capacity);
-  if ((long long)p->kv_heads * 2 * (p->slot_capacity / 8 + 2) > 0x7fffffffLL)
-    return set_error(PQHSA_E_SHAPE, "kv_heads * slot_capacity is too large");
+  if ((long long)p->requests * p->kv_heads * 2 * (p->slot_capacity / 8 + 2) > 0x7fffffffLL)
+    return set_error(PQHSA_E_SHAPE, "requests * kv_heads * slot_capacity must stay below 2^33");
   return PQHSA_OK;
 }
 
@@ -128,6 +130,7 @@ int pqhsa_paged_attention(const pqhsa_paged_params* p, void* stream) {
   a.part_acc = reinterpret_cast<float*>(ws + w.part_acc);
   a.row_lse2 = reinterpret_cast<float*>(ws + w.row_lse2);
   a.scores = p->mass != nullptr ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
+  a.score_stride = (int64_t)paged_score_stride(p->slot_capacity);
   return launch_paged_attend(a, p->dtype, (cudaStream_t)stream);
 }
 

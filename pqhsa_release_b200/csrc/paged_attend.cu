@@ -11,8 +11,9 @@
 // takes equal contiguous shares of it (paged.cuh).  Inside a CTA the tiles of a stream go to the warps in turn, each
 // with a ring of tiles in shared memory filled by 16-byte asynchronous copies; the warps' states are merged in shared
 // memory where a stream (or the share) ends.  A stream that lies in one share is finished there; of one that several
-// CTAs share, each writes (max, sum, acc), and the CTA whose ticket is the last folds them: no second launch, and no
-// CTA waits for another.
+// CTAs share (at most two of a CTA's streams: its first and its last), each writes (max, sum, acc) as it gets there
+// and takes a ticket when all its tiles are done; the CTA whose ticket is the last folds the parts: no second launch,
+// no CTA waits for another, and one fence a CTA.
 //
 // Keys that no row may see are not read at all: their rows in shared memory are filled with zeros, so whatever a page
 // holds there (NaN included) stays out.  A key that only some rows of the step see takes part with p = 0 for the
@@ -24,7 +25,11 @@ namespace pqhsa {
 constexpr int kPWarps = 8;
 constexpr int kPThreads = kPWarps * 32;
 constexpr float kLazy = 8.f;  // a running maximum is raised once a score passes it by 2^8: sums stay far from overflow
+constexpr float kFloor = -1.7e38f;  // the maximum before any key: finite, so that a score of -inf is p = 0 and not 2^NaN
 
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
 __device__ __forceinline__ void cp_async16_zfill(uint32_t smem, const void* gmem, bool take) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(take ? 16 : 0) : "memory");
 }
@@ -36,16 +41,17 @@ __device__ __forceinline__ float paged_score(const PagedArgs& a, float dot, floa
   return s;
 }
 
-// Ends a stream's part: the warps' (max, sum) in ml and accumulators in acc (rows of kAccStride floats) are merged and
-// written as output rows (the CTA had the whole stream) or as a partial.  All threads call; rows = rows of the pass.
-constexpr int kAccStride = kD + 4;
+// An element of a merge buffer [warps][rows][128]: the rows of a warp's accumulator layout in different banks.
+__device__ __forceinline__ int merge_at(int entry, int row, int rows, int dim) {
+  return (entry * rows + row) * kD + (dim ^ (((row >> 1) & 3) << 3));
+}
+
 template <typename E>
-__device__ __forceinline__ void paged_store_row(const PagedArgs& a, const PagedCursor& c, int row, int lane, float M, float L,
-                                                float4 o) {
-  const int pass = c.sub % a.groups, h = c.sub / a.groups, full = pass * kPagedGroupRows + row;
+__device__ __forceinline__ void paged_store_row(const PagedArgs& a, int r, int h, int pass, int row, int lane, float M, float L, float4 o) {
+  const int full = pass * kPagedGroupRows + row;
   const int t = full / a.G, hq = h * a.G + full % a.G;
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;  // an empty row is zero, a NaN stays one
-  E* dst = static_cast<E*>(a.out) + (int64_t)c.r * a.o_sr + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + lane * 4;
+  E* dst = static_cast<E*>(a.out) + (int64_t)r * a.o_sr + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + lane * 4;
   const E v[4] = {from_f<E>(o.x * inv), from_f<E>(o.y * inv), from_f<E>(o.z * inv), from_f<E>(o.w * inv)};
   if constexpr (sizeof(E) == 4) {
     *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(v);
@@ -54,151 +60,173 @@ __device__ __forceinline__ void paged_store_row(const PagedArgs& a, const PagedC
   }
   if (lane == 0) {
     const float l2 = L == 0.f ? kNegInf : M + log2f(L);
-    if (a.lse != nullptr) a.lse[((int64_t)c.r * a.T + t) * (a.H * a.G) + hq] = l2 * 0.69314718055994531f;
-    a.row_lse2[((int64_t)c.r * a.H + h) * a.R + full] = l2;
+    if (a.lse != nullptr) a.lse[((int64_t)r * a.T + t) * (a.H * a.G) + hq] = l2 * 0.69314718055994531f;
+    a.row_lse2[((int64_t)r * a.H + h) * a.R + full] = l2;
   }
 }
 
-template <typename E>
-__device__ void paged_finish(const PagedArgs& a, const PagedCursor& c, long long x0, int tile0, int tiles, long long total,
-                             int C, int rows, int pass_rows, const float2* ml, const float* acc, int* last_s) {
+// Running state of a row: o and L are relative to 2^M.  A part that has seen no key has M = kFloor, L = 0, o = 0.
+struct RowSum {
+  float M = kFloor, L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void raise(float m) {
+    const float to = fmaxf(M, m), f = ex2(M - to);
+    M = to;
+    L *= f;
+    o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+  }
+  __device__ __forceinline__ void add(float2 ml, const float4& v) {  // ml.x <= M
+    const float f = ex2(ml.x - M);
+    L = fmaf(ml.y, f, L);
+    o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+  }
+};
+
+// Streams this CTA has a part of, to be folded by the CTA that finishes the last of their parts.
+struct PagedPending {
+  int r, h, pass, c0, parts, last;
+};
+
+// Ends a stream in this share (all threads): the states of `entries` warps in ml [entries][ROWS] and acc are merged and
+// written as output rows (the share holds the whole stream) or as a part of it.
+template <typename E, int ROWS>
+__device__ __forceinline__ void paged_finish(const PagedArgs& a, const PagedShares& sh, const PagedCursor& c, int x, int count,
+                                             int rows, int entries, const float2* ml, const float* acc, PagedPending* pend) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool whole = tile0 == 0 && tiles == c.g.tiles;
-  const size_t part = (size_t)2 * blockIdx.x + (tile0 == 0 ? 1 : 0);  // at most one part of a CTA starts a stream it does not end
+  const bool starts = c.tile == 0, whole = starts && count == c.g.tiles;
+  const size_t part = (size_t)2 * blockIdx.x + (starts ? 1 : 0);
   for (int row = warp; row < rows; row += kPWarps) {
-    float M = kNegInf;
-#pragma unroll
-    for (int w = 0; w < kPWarps; ++w) M = fmaxf(M, ml[w * pass_rows + row].x);
-    float L = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kPWarps; ++w) {
-      const float2 x = ml[w * pass_rows + row];
-      if (x.x == kNegInf && x.y == 0.f) continue;  // this warp saw no key of the row
-      const float f = ex2(x.x - M);
-      const float4 v = *reinterpret_cast<const float4*>(acc + ((size_t)w * pass_rows + row) * kAccStride + lane * 4);
-      L = fmaf(x.y, f, L);
-      o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
-    }
+    RowSum s;
+    for (int w = 0; w < entries; ++w) s.M = fmaxf(s.M, ml[w * ROWS + row].x);
+    for (int w = 0; w < entries; ++w)
+      s.add(ml[w * ROWS + row], *reinterpret_cast<const float4*>(acc + merge_at(w, row, ROWS, lane * 4)));
     if (whole) {
-      paged_store_row<E>(a, c, row, lane, M, L, o);
+      paged_store_row<E>(a, c.r, c.h, c.pass, row, lane, s.M, s.L, s.o);
     } else {
-      if (lane == 0) a.part_ml[part * kPagedGroupRows + row] = make_float2(M, L);
-      *reinterpret_cast<float4*>(a.part_acc + (part * pass_rows + row) * kD + lane * 4) = o;
+      if (lane == 0) a.part_ml[part * kPagedGroupRows + row] = make_float2(s.M, s.L);
+      *reinterpret_cast<float4*>(a.part_acc + (part * ROWS + row) * kD + lane * 4) = s.o;
     }
   }
-  if (whole) return;
-  // the parts of a stream lie in CTAs c0 .. c1; the one whose ticket is the last folds them
-  const int c0 = (int)(((x0 + 1) * C - 1) / total), c1 = (int)(((x0 + c.g.tiles) * C - 1) / total);
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int seen = atomicAdd(a.tickets + c0, 1);
-    *last_s = seen == c1 - c0;
-    if (seen == c1 - c0) a.tickets[c0] = 0;
-  }
-  __syncthreads();
-  if (*last_s == 0) return;
-  __threadfence();
-  const int parts = c1 - c0 + 1;
-  for (int row = warp; row < rows; row += kPWarps) {
-    float M = kNegInf;
-    for (int s = lane; s < parts; s += 32) M = fmaxf(M, __ldcg(&a.part_ml[((size_t)2 * (c0 + s) + (s == 0)) * kPagedGroupRows + row].x));
-    M = warp_max(M);
-    float L = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int s = 0; s < parts; ++s) {
-      const size_t p = (size_t)2 * (c0 + s) + (s == 0);
-      const float2 x = __ldcg(&a.part_ml[p * kPagedGroupRows + row]);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_acc + (p * pass_rows + row) * kD + lane * 4));
-      const float f = x.x == kNegInf && x.y == 0.f ? 0.f : ex2(x.x - M);
-      L = fmaf(x.y, f, L);
-      o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y); o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
-    }
-    paged_store_row<E>(a, c, row, lane, M, L, o);
+  if (!whole && threadIdx.x == 0) {
+    PagedPending& p = pend[starts ? 1 : 0];
+    p.r = c.r;
+    p.h = c.h;
+    p.pass = c.pass;
+    p.c0 = sh.owner(x - c.tile);
+    p.parts = sh.owner(x - c.tile + c.g.tiles - 1) - p.c0 + 1;
   }
 }
 
-// ---- CUDA-core kernel: tiles of 8 keys -----------------------------------------------------------------
-// Scores: lane = (key, quarter of the dimensions); a quarter's lanes share the rows of the step for the softmax.
+// After the last tile of the CTA (all threads): tickets for its parts, and the fold of the streams it ends.
+template <typename E, int ROWS>
+__device__ __forceinline__ void paged_fold(const PagedArgs& a, PagedPending* pend, float2* ml, float* acc) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();  // the parts are written (by all threads) and pend is set
+  if (threadIdx.x == 0) {
+    if ((pend[0].parts | pend[1].parts) != 0) __threadfence();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      pend[i].last = 0;
+      if (pend[i].parts == 0) continue;
+      if (atomicAdd(a.tickets + pend[i].c0, 1) == pend[i].parts - 1) {
+        pend[i].last = 1;
+        a.tickets[pend[i].c0] = 0;
+      }
+    }
+    __threadfence();
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    if (pend[i].last == 0) continue;
+    const int parts = pend[i].parts, c0 = pend[i].c0, rows = min(a.R - pend[i].pass * kPagedGroupRows, kPagedGroupRows);
+    // warps of a row: all of them for one row, one for eight and more; each folds every per-th part
+    const int per = rows <= 1 ? kPWarps : rows <= 2 ? kPWarps / 2 : rows <= 4 ? kPWarps / 4 : 1;
+    const int at = warp % per;
+    for (int base = 0; base < rows; base += kPWarps / per) {
+      const int row = base + warp / per;
+      RowSum s;
+      if (row < rows) {
+        constexpr int kAhead = 8;  // loads in flight
+        for (int p0 = at; p0 < parts; p0 += kAhead * per) {
+          float2 x[kAhead];
+          float4 v[kAhead];
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            const int p = p0 + u * per;
+            const size_t place = (size_t)2 * (c0 + min(p, parts - 1)) + (min(p, parts - 1) == 0 ? 1 : 0);
+            x[u] = __ldcg(&a.part_ml[place * kPagedGroupRows + row]);
+            v[u] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + (place * ROWS + row) * kD + lane * 4));
+            if (p >= parts) {
+              x[u] = make_float2(kFloor, 0.f);
+              v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+          }
+          float top = x[0].x;
+#pragma unroll
+          for (int u = 1; u < kAhead; ++u) top = fmaxf(top, x[u].x);
+          s.raise(top);
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) s.add(x[u], v[u]);
+        }
+        if (per == 1) paged_store_row<E>(a, pend[i].r, pend[i].h, pend[i].pass, row, lane, s.M, s.L, s.o);
+      }
+      if (per == 1) continue;
+      __syncthreads();  // the buffer of the round before has been read
+      if (lane == 0) ml[warp] = make_float2(s.M, s.L);
+      *reinterpret_cast<float4*>(acc + warp * kD + lane * 4) = s.o;
+      __syncthreads();
+      if (at == 0 && row < rows) {
+        for (int w = warp + 1; w < warp + per; ++w) {
+          s.raise(ml[w].x);
+          s.add(ml[w], *reinterpret_cast<const float4*>(acc + w * kD + lane * 4));
+        }
+        paged_store_row<E>(a, pend[i].r, pend[i].h, pend[i].pass, row, lane, s.M, s.L, s.o);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---- fp32 caches: CUDA cores, tiles of 8 keys ---------------------------------------------------------------
+// Scores: lane = (key, quarter of the dimensions); a quarter's lanes look after every fourth row for the softmax.
 // Values: lane = 4 dimensions of all rows.  Row of a tile in shared memory: 16-byte pieces, piece j at j ^ (key & 7).
 constexpr int kKeys = 8;
 
-template <typename E> __device__ __forceinline__ const E* tile_piece(const E* tile, int key, int elem) {
-  constexpr int n = 16 / sizeof(E);  // elements of a piece; elem is a multiple of 4
-  const int piece = elem / n;
-  return tile + key * kD + ((piece ^ (key & 7)) * n) + elem % n;
-}
-__device__ __forceinline__ void tile4(const float* p, float (&v)[4]) {
-  const float4 x = *reinterpret_cast<const float4*>(p);
-  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-}
-template <typename E> __device__ __forceinline__ void tile4(const E* p, float (&v)[4]) {
-  unpack4(*reinterpret_cast<const uint2*>(p), static_cast<const E*>(nullptr), v);
+__device__ __forceinline__ float4 tile_piece(const float* tile, int key, int elem) {  // elem: a multiple of 4
+  return *reinterpret_cast<const float4*>(tile + key * kD + (((elem >> 2) ^ (key & 7)) << 2));
 }
 
-template <typename E, int ROWS, int STAGES>
+template <int ROWS, int STAGES>
 __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedArgs a) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr int kStage = 2 * kKeys * kD;  // elements of a stage: 8 key rows, then 8 value rows
-  E* ring = reinterpret_cast<E*>(smem_raw) + (threadIdx.x >> 5) * (STAGES * kStage);
+  constexpr int OWN = ROWS / 4;
+  float* ring = reinterpret_cast<float*>(smem_raw) + (threadIdx.x >> 5) * (STAGES * kStage);
   float* acc_s = reinterpret_cast<float*>(smem_raw);  // merge buffer over the rings, used between streams
-  constexpr size_t kRing = sizeof(E) * kPWarps * STAGES * kStage;
-  constexpr size_t kMerge = sizeof(float) * kPWarps * ROWS * kAccStride;
-  uint8_t* tail = smem_raw + (kRing > kMerge ? kRing : kMerge);
-  float* q_s = reinterpret_cast<float*>(tail);                                   // [ROWS][128]
-  float* p_s = q_s + ROWS * kD + (threadIdx.x >> 5) * (ROWS * kKeys);             // per warp [ROWS][8]
+  static_assert(ROWS <= 2 * STAGES * kKeys, "the merge buffer fits the rings");
+  float* q_s = reinterpret_cast<float*>(smem_raw) + kPWarps * STAGES * kStage;         // [ROWS][128]
+  float* p_s = q_s + ROWS * kD + (threadIdx.x >> 5) * (ROWS * kKeys);                  // per warp [ROWS][8]
   float2* ml_s = reinterpret_cast<float2*>(q_s + ROWS * kD + kPWarps * ROWS * kKeys);  // [warps][ROWS]
   __shared__ int pos_s[kPWarps][STAGES][kKeys];
-  __shared__ int seen_s[kPWarps][STAGES];
-  __shared__ int last_s;
+  __shared__ int seen_s[kPWarps][STAGES];  // keys some row of the step sees; << 16: keys not all of them see
+  __shared__ PagedPending pend_s[2];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int key = lane & 7, quarter = lane >> 3;
-  constexpr int OWN = ROWS / 4;
-  const E* kb = static_cast<const E*>(a.k_base);
-  const E* vb = static_cast<const E*>(a.v_base);
+  const float* kb = static_cast<const float*>(a.k_base);
+  const float* vb = static_cast<const float*>(a.v_base);
 
-  const long long total = paged_total(a);
-  const int C = (int)min((long long)gridDim.x, total);  // CTAs with a share: none of them is empty
-  if (blockIdx.x >= C) return;
-  long long x = paged_share(total, blockIdx.x, C);
-  const long long x_end = paged_share(total, blockIdx.x + 1, C);
-  PagedCursor c = paged_locate(a, x);
+  PagedCursor c;
+  const PagedShares sh = paged_locate(a, gridDim.x, blockIdx.x, c);
+  if (blockIdx.x >= sh.C) return;
+  int x = sh.first(blockIdx.x);
+  const int x_end = sh.first(blockIdx.x + 1);
+  if (tid < 2) pend_s[tid].parts = 0;
 
   while (true) {
-    const int count = (int)min((long long)(c.g.tiles - c.tile), x_end - x);  // tiles of this stream in the share
-    const int pass = c.sub % a.groups, h = c.sub / a.groups;
-    const int row0 = pass * kPagedGroupRows, rows = min(a.R - row0, kPagedGroupRows);
-    __syncthreads();  // the merge buffer and q_s are free again
-    for (int i = tid; i < ROWS * (kD / 4); i += kPThreads) {
-      const int row = i / (kD / 4), d = i % (kD / 4) * 4;
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-      if (row < rows) {
-        const int full = row0 + row;
-        load4(static_cast<const E*>(a.q) + (int64_t)c.r * a.q_sr + (int64_t)(full / a.G) * a.q_st +
-                  (int64_t)(h * a.G + full % a.G) * a.q_sh + d, v);
-      }
-      *reinterpret_cast<float4*>(q_s + row * kD + d) = make_float4(v[0], v[1], v[2], v[3]);
-    }
-    float slope[OWN], m[OWN], l[OWN], acc[ROWS][4];
-    int p_at[OWN];
-#pragma unroll
-    for (int i = 0; i < OWN; ++i) {
-      const int full = row0 + 4 * i + quarter;
-      const bool live = 4 * i + quarter < rows;
-      p_at[i] = live ? c.g.p_first + full / a.G : -1;
-      slope[i] = live && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + full % a.G) : 0.f;
-      m[i] = kNegInf;
-      l[i] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-    __syncthreads();
-
+    const int count = min(c.g.tiles - c.tile, x_end - x);  // tiles of this stream in the share
+    const int h = c.h, row0 = c.pass * kPagedGroupRows, rows = min(a.R - row0, kPagedGroupRows);
     const int mine = count > warp ? (count - warp + kPWarps - 1) / kPWarps : 0;
     const int32_t* kpos = a.key_pos != nullptr ? a.key_pos + ((int64_t)c.r * a.H + h) * a.cap : nullptr;
     // fills ring slot `st` with tile number `it` of this warp
@@ -211,48 +239,69 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
           off = paged_offset(a, c.r, h, slot);
           pos = kpos != nullptr ? __ldg(kpos + slot) : slot;
         }
-        bool any = off >= 0 && pos >= c.g.first && pos <= c.g.p_last;
-        if (any && a.window > 0) any = c.g.p_first - pos < a.window || pos - c.g.first < a.sinks;
-        const unsigned seen = __ballot_sync(0xffffffffu, any) & 0xffu;
+        const PagedSight v = paged_sight(c.g, a, off >= 0, pos);
+        const unsigned seen = __ballot_sync(0xffffffffu, v.any) & 0xffu, mixed = __ballot_sync(0xffffffffu, v.any && !v.all) & 0xffu;
         if (lane < kKeys) pos_s[warp][st][lane] = pos;
-        if (lane == 0) seen_s[warp][st] = (int)seen;
-        // a row is kD * sizeof(E) / 16 pieces: 32 lanes cover 1 (fp32) or 2 (16-bit) rows at a time
-        constexpr int pieces = kD * (int)sizeof(E) / 16, at_once = 32 / pieces;
-        E* dst = ring + st * kStage;
+        if (lane == 0) seen_s[warp][st] = (int)(seen | mixed << 16);
+        float* dst = ring + st * kStage;
 #pragma unroll
-        for (int r = 0; r < kKeys; r += at_once) {
-          const int k = r + lane / pieces, piece = lane % pieces;
+        for (int k = 0; k < kKeys; ++k) {  // a row is 32 pieces of 16 bytes: one a lane
           const int64_t o = __shfl_sync(0xffffffffu, off, k);
           const bool take = (seen >> k) & 1u;
-          const int64_t e = (take ? o : 0) + piece * (16 / (int)sizeof(E));
-          const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + k * kD + (piece ^ (k & 7)) * (16 / (int)sizeof(E)));
+          const int64_t e = (take ? o : 0) + lane * 4;
+          const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst + k * kD + ((lane ^ k) << 2));
           cp_async16_zfill(to, kb + e, take);
-          cp_async16_zfill(to + kKeys * kD * sizeof(E), vb + e, take);
+          cp_async16_zfill(to + kKeys * kD * 4, vb + e, take);
         }
       }
       cp_async_commit();
     };
+    __syncthreads();  // the merge buffer and q_s are free again
 #pragma unroll
     for (int st = 0; st < STAGES - 1; ++st) load(st, st);
+    for (int i = tid; i < ROWS * (kD / 4); i += kPThreads) {
+      const int row = i / (kD / 4), d = i % (kD / 4) * 4, full = row0 + row;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row < rows)
+        v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)c.r * a.q_sr + (int64_t)(full / a.G) * a.q_st +
+                                                  (int64_t)(h * a.G + full % a.G) * a.q_sh + d));
+      *reinterpret_cast<float4*>(q_s + row * kD + d) = v;
+    }
+    float slope[OWN], m[OWN], l[OWN], acc[ROWS][4];
+    int p_at[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const int full = row0 + 4 * i + quarter;
+      const bool live = 4 * i + quarter < rows;
+      p_at[i] = live ? c.g.p_first + full / a.G : -1;
+      slope[i] = live && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + full % a.G) : 0.f;
+      m[i] = kFloor;
+      l[i] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    __syncthreads();
+
     for (int it = 0; it < mine; ++it) {
       const int st = it % STAGES;
       cp_async_wait<STAGES - 2>();
       __syncwarp();
       load(it + STAGES - 1, (it + STAGES - 1) % STAGES);
-      const E* kt = ring + st * kStage;
-      const E* vt = kt + kKeys * kD;
+      const float* kt = ring + st * kStage;
+      const float* vt = kt + kKeys * kD;
       float s[ROWS];
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) s[i] = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {  // 32 dimensions of a quarter, 4 at a time, each quarter in its own order (banks)
         const int d = quarter * 32 + ((j ^ (2 * quarter)) & 7) * 4;
-        float kv[4];
-        tile4(tile_piece(kt, key, d), kv);
+        const float4 kv = tile_piece(kt, key, d);
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
           const float4 qv = *reinterpret_cast<const float4*>(q_s + i * kD + d);
-          s[i] = fmaf(kv[0], qv.x, fmaf(kv[1], qv.y, fmaf(kv[2], qv.z, fmaf(kv[3], qv.w, s[i]))));
+          s[i] = fmaf(kv.x, qv.x, fmaf(kv.y, qv.y, fmaf(kv.z, qv.z, fmaf(kv.w, qv.w, s[i]))));
         }
       }
 #pragma unroll
@@ -261,7 +310,8 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
         s[i] += __shfl_xor_sync(0xffffffffu, s[i], 16);
       }
       const int pos = pos_s[warp][st][key];
-      const bool here = (seen_s[warp][st] >> key) & 1;
+      const unsigned flags = (unsigned)seen_s[warp][st];
+      const bool here = (flags >> key) & 1u;
       float own[OWN];
       bool raise = false;
 #pragma unroll
@@ -272,11 +322,11 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
       }
       if (a.scores != nullptr) {
         const int slot = paged_tile(c.g, c.tile + warp + it * kPWarps) * kKeys + key;
-        float* dst = a.scores + (((int64_t)c.r * a.H + h) * a.R + row0) * a.cap + slot;
+        float* dst = a.scores + (((int64_t)c.r * a.H + h) * a.R + row0) * a.score_stride + slot;
         if (slot < c.g.n) {
 #pragma unroll
           for (int i = 0; i < OWN; ++i)
-            if (4 * i + quarter < rows) dst[(int64_t)(4 * i + quarter) * a.cap] = own[i];
+            if (4 * i + quarter < rows) dst[(int64_t)(4 * i + quarter) * a.score_stride] = own[i];
         }
       }
       if (__any_sync(0xffffffffu, raise)) {
@@ -286,7 +336,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           const float to = fmaxf(m[i], top);
-          const float f = m[i] == kNegInf ? (to == kNegInf ? 1.f : 0.f) : ex2(m[i] - to);
+          const float f = ex2(m[i] - to);
           m[i] = to;
           l[i] *= f;
 #pragma unroll
@@ -300,24 +350,29 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
       __syncwarp();  // p_s of the tile before has been read
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
-        const float p = own[i] == kNegInf ? 0.f : ex2(own[i] - m[i]);
+        const float p = ex2(own[i] - m[i]);
         l[i] += p;
         p_s[(4 * i + quarter) * kKeys + key] = p;
       }
       __syncwarp();
+      const bool guard = (flags >> 16) != 0u;  // a key that only some rows see: its value is multiplied only where p is not 0
 #pragma unroll
       for (int k4 = 0; k4 < kKeys; k4 += 4) {
-        float v[4][4];
+        float4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) tile4(tile_piece(vt, k4 + k, lane * 4), v[k]);
+        for (int k = 0; k < 4; ++k) v[k] = tile_piece(vt, k4 + k, lane * 4);
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
           const float4 p = *reinterpret_cast<const float4*>(p_s + i * kKeys + k4);
           const float pk[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = pk[k] != 0.f ? fmaf(pk[k], v[k][j], acc[i][j]) : acc[i][j];
+          for (int k = 0; k < 4; ++k) {
+            if (guard && pk[k] == 0.f) continue;
+            acc[i][0] = fmaf(pk[k], v[k].x, acc[i][0]);
+            acc[i][1] = fmaf(pk[k], v[k].y, acc[i][1]);
+            acc[i][2] = fmaf(pk[k], v[k].z, acc[i][2]);
+            acc[i][3] = fmaf(pk[k], v[k].w, acc[i][3]);
+          }
         }
       }
       __syncwarp();  // the slot may be filled again
@@ -332,24 +387,22 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
     }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
-      *reinterpret_cast<float4*>(acc_s + ((size_t)warp * ROWS + i) * kAccStride + lane * 4) =
-          make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+      *reinterpret_cast<float4*>(acc_s + merge_at(warp, i, ROWS, lane * 4)) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
     __syncthreads();
-    paged_finish<E>(a, c, x - c.tile, c.tile, count, total, C, rows, ROWS, ml_s, acc_s, &last_s);
+    paged_finish<float, ROWS>(a, sh, c, x, count, rows, kPWarps, ml_s, acc_s, pend_s);
     x += count;
-    if (x >= x_end) return;
+    if (x >= x_end) break;
     paged_next_stream(a, c);
   }
+  paged_fold<float, ROWS>(a, pend_s, ml_s, acc_s);
 }
 
-template <typename E, int ROWS, int STAGES>
-static int launch_simple(const PagedArgs& a, cudaStream_t st) {
-  constexpr size_t ring = sizeof(E) * kPWarps * STAGES * 2 * kKeys * kD;
-  constexpr size_t merge = sizeof(float) * kPWarps * ROWS * kAccStride;
-  constexpr size_t smem = (ring > merge ? ring : merge) + sizeof(float) * (ROWS * kD + kPWarps * ROWS * kKeys) +
+template <int ROWS, int STAGES>
+static int launch_fp32(const PagedArgs& a, cudaStream_t st) {
+  constexpr size_t smem = sizeof(float) * (kPWarps * STAGES * 2 * kKeys * kD + ROWS * kD + kPWarps * ROWS * kKeys) +
                           sizeof(float2) * kPWarps * ROWS;
-  static_assert(smem <= 220 * 1024, "shared memory of a CTA");
-  auto kern = paged_attend_kernel<E, ROWS, STAGES>;
+  static_assert(smem <= 225 * 1024, "shared memory of a CTA");
+  auto kern = paged_attend_kernel<ROWS, STAGES>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return check_launch("paged_attend shared memory");
   kern<<<sm_count(), kPThreads, smem, st>>>(a);
@@ -402,109 +455,129 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// A warp's view of the tiles it has still to fetch: lane i < 16 looks after key i.  What the addresses depend on (page
-// table, stored positions) is requested one tile before it is needed.
-struct TileFetch {
-  int32_t entry;  // page
-  int32_t row;    // row in the page
-  int32_t pos;    // position, or a value no token sees
-};
-
-template <typename E, int NB, int STAGES>
+// The copies run ahead of the products across the ends of streams: a warp's tiles of all its CTA's streams form one
+// sequence, which `ahead` walks STAGES - 1 tiles in front of `c`; the merge of a stream's warps has its own buffer, so
+// the ring stays full meanwhile.  What a tile's addresses depend on (page table, stored positions) is asked for one tile
+// before the tile itself.  SHAPED: scores have a cap or a distance bias.
+template <typename E, int NB, int STAGES, bool SHAPED>
 __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const PagedArgs a) {
   constexpr int ROWS = 8 * NB;
   constexpr bool QREG = NB <= 2;  // query rows as B fragments in registers; from shared memory when they would fill them
   constexpr int kStageB = 2 * kMKeys * kD * 2;  // bytes of a stage: 16 key rows, then 16 value rows, 256 bytes each
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  constexpr size_t kRing = (size_t)kPWarps * STAGES * kStageB;
-  constexpr size_t kMerge = sizeof(float) * kPWarps * ROWS * kAccStride;
-  float* acc_s = reinterpret_cast<float*>(smem_raw);  // merge buffer over the rings, used between streams
-  uint8_t* tail = smem_raw + (kRing > kMerge ? kRing : kMerge);
-  float2* ml_s = reinterpret_cast<float2*>(tail);                 // [warps][ROWS]
-  uint8_t* q_s = tail + sizeof(float2) * kPWarps * ROWS;          // [ROWS][128] E, pieces swizzled, only without QREG
+  constexpr int kHalf = kPWarps / 2;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  float* acc_s = reinterpret_cast<float*>(smem_raw + (size_t)kPWarps * STAGES * kStageB);  // merge buffer [warps / 2][ROWS][128]
+  float2* ml_s = reinterpret_cast<float2*>(acc_s + kHalf * ROWS * kD);                     // [warps][ROWS]
+  uint8_t* q_s = reinterpret_cast<uint8_t*>(ml_s + kPWarps * ROWS);                        // [ROWS][128] E, swizzled, only without QREG
   __shared__ int pos_s[kPWarps][STAGES][kMKeys];
   __shared__ int seen_s[kPWarps][STAGES];   // keys some row of the step sees; << 16: keys not all of them see
-  __shared__ int last_s;
+  __shared__ PagedPending pend_s[2];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t4 = lane & 3, l4 = lane >> 2;
   const E* kb = static_cast<const E*>(a.k_base);
   const E* vb = static_cast<const E*>(a.v_base);
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem_raw) + warp * (STAGES * kStageB);
-  // shared-memory addresses inside a tile, before the 16-byte piece is added: piece j of row k lies at j ^ (k & 7)
-  const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_hi = lane >> 4;          // K: rows 0-7 | 8-15, then the upper 8 dims
-  const int v_row = (lane & 7) + (lane >> 4) * 8, v_hi = (lane >> 3) & 1;          // V: upper 8 dims, then rows 8-15
-  const int g_row = lane >> 3, g_piece = lane & 7;                                 // copies: 4 rows x 128 bytes at a time
+  // Lane's addresses inside a tile.  Piece j of row k lies at j ^ (k & 7): an even piece 2 i further on is the address
+  // with i << 5 exclusive-ored in, as tiles start on 256-byte boundaries.
+  const int k_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_row = (lane & 7) + (lane >> 4) * 8;  // K: rows 0-7 | 8-15, then the
+  const uint32_t k_lane = ring + k_row * 256 + ((((uint32_t)lane >> 4) ^ (k_row & 7)) << 4);    // upper 8 dims; V: the upper 8
+  const uint32_t v_lane = ring + (kMKeys + v_row) * 256 + (((((uint32_t)lane >> 3) & 1) ^ (v_row & 7)) << 4);  // dims, then rows 8-15
+  const int g_row = lane >> 3, g_piece = lane & 7;                                              // copies: 4 rows x 128 bytes at a time
+  const uint32_t g_lane = ring + g_row * 256 + ((g_piece ^ g_row) << 4);
 
-  const long long total = paged_total(a);
-  const int C = (int)min((long long)gridDim.x, total);  // CTAs with a share: none of them is empty
-  if (blockIdx.x >= C) return;
-  long long x = paged_share(total, blockIdx.x, C);
-  const long long x_end = paged_share(total, blockIdx.x + 1, C);
-  PagedCursor c = paged_locate(a, x);
+  PagedCursor c;
+  const PagedShares sh = paged_locate(a, gridDim.x, blockIdx.x, c);
+  if (blockIdx.x >= sh.C) return;
+  int x = sh.first(blockIdx.x);
+  const int x_end = sh.first(blockIdx.x + 1);
+  if (tid < 2) pend_s[tid].parts = 0;
 
-  while (true) {
-    const int count = (int)min((long long)(c.g.tiles - c.tile), x_end - x);  // tiles of this stream in the share
-    const int pass = c.sub % a.groups, h = c.sub / a.groups;
-    const int row0 = pass * kPagedGroupRows, rows = min(a.R - row0, kPagedGroupRows);
-    const int mine = count > warp ? (count - warp + kPWarps - 1) / kPWarps : 0;
-    const int32_t* kpos = a.key_pos != nullptr ? a.key_pos + ((int64_t)c.r * a.H + h) * a.cap : nullptr;
-    const int32_t* table = a.block_table != nullptr ? a.block_table + (int64_t)c.r * a.max_blocks : nullptr;
-
-    auto fetch = [&](int it) {
-      TileFetch f = {-1, 0, -1};
-      if (it < mine && lane < kMKeys) {
-        const int slot = paged_tile(c.g, c.tile + warp + it * kPWarps) * kMKeys + lane;
-        if (slot < c.g.n) {
-          f.pos = kpos != nullptr ? __ldg(kpos + slot) : slot;
-          f.entry = c.r;
-          f.row = slot;
-          if (table != nullptr) {
-            const int b = slot / a.block_size;
-            f.row = slot - b * a.block_size;
-            f.entry = __ldg(table + b);
-          }
-        }
+  // the copies' cursor: tile number `at` of the `at_end` of this warp in stream `ahead`
+  PagedCursor ahead = c;
+  int ahead_x = x;
+  auto tiles_of = [&](int count) { return count > warp ? (count - warp + kPWarps - 1) / kPWarps : 0; };
+  int at = 0, at_end = tiles_of(min(ahead.g.tiles - ahead.tile, x_end - ahead_x));
+  bool more = true;
+  // a tile of whole pages or of a contiguous cache lies in one piece: its rows are stride_row apart
+  const bool even = a.block_table == nullptr || a.block_size % kMKeys == 0;
+  // next tile, and for each lane the page of key (lane & 15), its row there and its position (one no token sees: -1)
+  int n_slot0 = 0, n_entry = -1, n_row = 0, n_pos = -1;
+  auto fetch = [&]() {
+    while (at == at_end) {  // on to the next stream in which this warp has a tile
+      ahead_x += min(ahead.g.tiles - ahead.tile, x_end - ahead_x);
+      if (ahead_x >= x_end) {
+        more = false;
+        return;
       }
-      return f;
-    };
-    auto load = [&](int it, int st, const TileFetch& f) {
-      if (it < mine) {
-        bool any = f.entry >= 0 && f.entry < a.num_blocks && f.pos >= c.g.first && f.pos <= c.g.p_last;
-        bool all = f.pos <= c.g.p_first;
-        if (a.window > 0) {
-          const bool sink = f.pos - c.g.first < a.sinks;
-          any = any && (c.g.p_first - f.pos < a.window || sink);
-          all = all && (c.g.p_last - f.pos < a.window || sink);
-        }
-        const unsigned seen = __ballot_sync(0xffffffffu, any), mixed = __ballot_sync(0xffffffffu, any && !all);
-        if (lane < kMKeys) pos_s[warp][st][lane] = f.pos;
-        if (lane == 0) seen_s[warp][st] = (int)((seen & 0xffffu) | (mixed << 16));
-        const int64_t off = any ? f.entry * a.stride_block + h * a.stride_head + f.row * a.stride_row : 0;
-        const uint32_t dst = ring + st * kStageB;
+      paged_next_stream(a, ahead);
+      at = 0;
+      at_end = tiles_of(min(ahead.g.tiles, x_end - ahead_x));
+    }
+    n_slot0 = paged_tile(ahead.g, ahead.tile + warp + at * kPWarps) * kMKeys;
+    ++at;
+    const int slot = n_slot0 + (lane & (kMKeys - 1));
+    n_entry = ahead.r;
+    n_row = slot;
+    n_pos = slot;
+    const bool there = slot < ahead.g.n;
+    if (!there) n_pos = n_entry = -1;
+    if (a.key_pos != nullptr && there) n_pos = __ldg(a.key_pos + ((int64_t)ahead.r * a.H + ahead.h) * a.cap + slot);
+    if (a.block_table != nullptr) {
+      const int b = (unsigned)slot / (unsigned)a.block_size;
+      n_row = slot - b * a.block_size;
+      if (there) n_entry = __ldg(a.block_table + (int64_t)ahead.r * a.max_blocks + b);
+    }
+  };
+  auto load = [&](int st) {  // `ahead` is still in the tile's stream
+    if (more) {
+      const PagedGeom& g = ahead.g;
+      const bool page = n_entry >= 0 && n_entry < a.num_blocks;
+      const PagedSight v = paged_sight(g, a, page, n_pos);
+      const unsigned seen = __ballot_sync(0xffffffffu, v.any) & 0xffffu, mixed = __ballot_sync(0xffffffffu, v.any && !v.all) << 16;
+      if (lane < kMKeys) pos_s[warp][st][lane] = n_pos;
+      if (lane == 0) seen_s[warp][st] = (int)(seen | mixed);
+      const int64_t off = (page ? n_entry : 0) * a.stride_block + ahead.h * a.stride_head + (int64_t)n_row * a.stride_row;
+      const uint32_t to = g_lane + st * kStageB;
+      if (even && seen == 0xffffu) {
+        const int64_t step = 4 * a.stride_row;
+        int64_t o = __shfl_sync(0xffffffffu, off, g_row) + g_piece * 8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int k = 4 * i + g_row;
-          const int64_t o = __shfl_sync(0xffffffffu, off, k) + g_piece * 8;
-          const bool take = (seen >> k) & 1u;
-          const uint32_t to = dst + k * 256 + ((g_piece ^ (k & 7)) << 4);
+        for (int i = 0; i < 4; ++i, o += step) {
+          const E* kr = kb + o;
+          const E* vr = vb + o;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            cp_async16_zfill(to + j * 128, kb + o + j * 64, take);
-            cp_async16_zfill(to + j * 128 + kMKeys * 256, vb + o + j * 64, take);
+            cp_async16((to ^ ((i & 1) << 6)) + i * 1024 + j * 128, kr + j * 64);
+            cp_async16((to ^ ((i & 1) << 6)) + i * 1024 + j * 128 + kMKeys * 256, vr + j * 64);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, 4 * i + g_row) + g_piece * 8;
+          const bool take = (seen >> (4 * i + g_row)) & 1u;
+          const E* kr = kb + (take ? o : 0);
+          const E* vr = vb + (take ? o : 0);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            cp_async16_zfill((to ^ ((i & 1) << 6)) + i * 1024 + j * 128, kr + j * 64, take);
+            cp_async16_zfill((to ^ ((i & 1) << 6)) + i * 1024 + j * 128 + kMKeys * 256, vr + j * 64, take);
           }
         }
       }
-      cp_async_commit();
-    };
+    }
+    cp_async_commit();
+  };
 
-    uint32_t qf[QREG ? NB : 1][8][2];
-    if constexpr (!QREG) __syncthreads();  // q_s of the stream before has been read
+  uint32_t qf[QREG ? NB : 1][8][2];
+  auto load_q = [&](const PagedCursor& s) {
+    const int row0 = s.pass * kPagedGroupRows, rows = min(a.R - row0, kPagedGroupRows);
+    const E* base = static_cast<const E*>(a.q) + (int64_t)s.r * a.q_sr + (int64_t)s.h * a.G * a.q_sh;
     if constexpr (QREG) {
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const int row = 8 * nb + l4, full = row0 + row;
-        const E* src = static_cast<const E*>(a.q) + (int64_t)c.r * a.q_sr + (int64_t)(full / a.G) * a.q_st +
-                       (int64_t)(h * a.G + full % a.G) * a.q_sh + 2 * t4;
+        const E* src = base + (int64_t)(full / a.G) * a.q_st + (int64_t)(full % a.G) * a.q_sh + 2 * t4;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
           qf[nb][kk][0] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
@@ -516,19 +589,26 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
         const int row = i >> 4, piece = i & 15, full = row0 + row;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (row < rows)
-          v = __ldg(reinterpret_cast<const uint4*>(static_cast<const E*>(a.q) + (int64_t)c.r * a.q_sr +
-                                                   (int64_t)(full / a.G) * a.q_st + (int64_t)(h * a.G + full % a.G) * a.q_sh) + piece);
+          v = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)(full / a.G) * a.q_st + (int64_t)(full % a.G) * a.q_sh) + piece);
         *reinterpret_cast<uint4*>(q_s + row * 256 + ((piece ^ (row & 7)) << 4)) = v;
       }
       __syncthreads();
     }
-    TileFetch next = fetch(0);
+  };
+
+  fetch();
 #pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) {
-      const TileFetch f = next;
-      next = fetch(st + 1);
-      load(st, st, f);
-    }
+  for (int st = 0; st < STAGES - 1; ++st) {
+    load(st);
+    fetch();
+  }
+  load_q(c);
+  int st = 0;  // ring slot of the next tile
+
+  while (true) {
+    const int count = min(c.g.tiles - c.tile, x_end - x);  // tiles of this stream in the share
+    const int mine = tiles_of(count);
+    const int h = c.h, row0 = c.pass * kPagedGroupRows, rows = min(a.R - row0, kPagedGroupRows);
     float m[NB][2], l[NB][2], slope[NB][2], o[NB][8][4];
     int p_at[NB][2];
 #pragma unroll
@@ -536,10 +616,10 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int row = 8 * nb + 2 * t4 + j, full = row0 + row;
-        m[nb][j] = kNegInf;
+        m[nb][j] = kFloor;
         l[nb][j] = 0.f;
         p_at[nb][j] = row < rows ? c.g.p_first + full / a.G : -1;
-        slope[nb][j] = row < rows && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + full % a.G) : 0.f;
+        slope[nb][j] = SHAPED && row < rows && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + full % a.G) : 0.f;
       }
 #pragma unroll
       for (int db = 0; db < 8; ++db)
@@ -548,15 +628,11 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
     }
 
     for (int it = 0; it < mine; ++it) {
-      const int st = it % STAGES;
       cp_async_wait<STAGES - 2>();
-      __syncwarp();
-      {
-        const TileFetch f = next;
-        next = fetch(it + STAGES);
-        load(it + STAGES - 1, (it + STAGES - 1) % STAGES, f);
-      }
-      const uint32_t kt = ring + st * kStageB, vt = kt + kMKeys * 256;
+      __syncwarp();  // the tile has landed, and the slot before it may be filled again
+      load(st == 0 ? STAGES - 1 : st - 1);
+      fetch();
+      const uint32_t kt = k_lane + st * kStageB, vt = v_lane + st * kStageB;
       float s[NB][4];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
@@ -565,8 +641,8 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
 #pragma unroll
       for (int kk = 0; kk < 8; kk += 2) {
         uint32_t a0[4], a1[4];
-        ldmatrix4(a0, kt + k_row * 256 + (((2 * kk + k_hi) ^ (k_row & 7)) << 4));
-        ldmatrix4(a1, kt + k_row * 256 + (((2 * kk + 2 + k_hi) ^ (k_row & 7)) << 4));
+        ldmatrix4(a0, kt ^ (kk << 5));
+        ldmatrix4(a1, kt ^ ((kk + 1) << 5));
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           if constexpr (QREG) {
@@ -581,32 +657,45 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
           }
         }
       }
-      // s[nb][0], [1]: key l4, rows 2 t4 and 2 t4 + 1 of block nb; [2], [3]: key l4 + 8
+      // s[nb][0], [1]: key l4, rows 2 t4 and 2 t4 + 1 of block nb; [2], [3]: key l4 + 8.  Rows past the step's are not
+      // masked: their query is 0 and nothing of them is written.
       const unsigned flags = (unsigned)seen_s[warp][st];
-      const int pos0 = pos_s[warp][st][l4], pos1 = pos_s[warp][st][l4 + 8];
-      const bool seen0 = (flags >> l4) & 1u, seen1 = (flags >> (l4 + 8)) & 1u;
       const unsigned mixed = flags >> 16;
+      if constexpr (SHAPED) {
+        const int pos0 = pos_s[warp][st][l4], pos1 = pos_s[warp][st][l4 + 8];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            s[nb][j] = paged_score(a, s[nb][j], slope[nb][j & 1], p_at[nb][j & 1] - (j < 2 ? pos0 : pos1));
+      } else {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[nb][j] *= a.scale_log2;
+      }
+      if (flags != 0xffffu) {
+        const int pos0 = pos_s[warp][st][l4], pos1 = pos_s[warp][st][l4 + 8];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (((flags >> (j < 2 ? l4 : l4 + 8)) & 1u) == 0u || !paged_sees(c.g, a, j < 2 ? pos0 : pos1, p_at[nb][j & 1])) s[nb][j] = kNegInf;
+      }
       bool raise = false;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int pos = j < 2 ? pos0 : pos1, p = p_at[nb][j & 1];
-          bool vis = (j < 2 ? seen0 : seen1) && p >= 0;
-          if (mixed != 0u) vis = vis && paged_sees(c.g, a, pos, p);
-          s[nb][j] = vis ? paged_score(a, s[nb][j], slope[nb][j & 1], p - pos) : kNegInf;
-          raise |= s[nb][j] > m[nb][j & 1] + kLazy;
-        }
-      }
+        for (int j = 0; j < 4; ++j) raise |= s[nb][j] > m[nb][j & 1] + kLazy;
       if (a.scores != nullptr) {
         const int slot = paged_tile(c.g, c.tile + warp + it * kPWarps) * kMKeys + l4;
-        float* dst = a.scores + (((int64_t)c.r * a.H + h) * a.R + row0 + 2 * t4) * a.cap + slot;
+        float* dst = a.scores + (((int64_t)c.r * a.H + h) * a.R + row0 + 2 * t4) * a.score_stride + slot;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (8 * nb + 2 * t4 + (j & 1) < rows && slot + (j >> 1) * 8 < c.g.n)
-              dst[(int64_t)(8 * nb + (j & 1)) * a.cap + (j >> 1) * 8] = s[nb][j];
+              dst[(int64_t)(8 * nb + (j & 1)) * a.score_stride + (j >> 1) * 8] = s[nb][j];
       }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -617,7 +706,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const float to = fmaxf(m[nb][j], top);
-            const float f = m[nb][j] == kNegInf ? (to == kNegInf ? 1.f : 0.f) : ex2(m[nb][j] - to);
+            const float f = ex2(m[nb][j] - to);
             m[nb][j] = to;
             l[nb][j] *= f;
 #pragma unroll
@@ -631,13 +720,13 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[nb][j] = s[nb][j] == kNegInf ? 0.f : ex2(s[nb][j] - m[nb][j & 1]);
+          s[nb][j] = ex2(s[nb][j] - m[nb][j & 1]);
           l[nb][j & 1] += s[nb][j];
         }
       if (mixed != 0u) {
         // Keys that only some rows see (at most the last query_len - 1 and as many at the window's edge): a product with
         // p = 0 would let an infinite or NaN value through, so these are added one by one and then taken out.
-        uint8_t* vrow = smem_raw + (vt - (uint32_t)__cvta_generic_to_shared(smem_raw));
+        uint8_t* vrow = smem_raw + ((size_t)(warp * STAGES + st) * 2 + 1) * (kMKeys * 256);
         unsigned left = mixed;
         while (left != 0u) {
           const int k = __ffs(left) - 1;
@@ -674,45 +763,82 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
         uint32_t av[4];
-        ldmatrix4_trans(av, vt + v_row * 256 + (((2 * db + v_hi) ^ (v_row & 7)) << 4));
+        ldmatrix4_trans(av, vt ^ (db << 5));
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) mma16816<E>(o[nb][db], av, pf[nb][0], pf[nb][1]);
       }
-      __syncwarp();  // the slot may be filled again
+      st = st + 1 == STAGES ? 0 : st + 1;
     }
-    cp_async_wait<0>();
-    __syncthreads();  // every warp is done with its ring: the merge buffer lies over it
+
+    // the stream's end in this share: the upper warps hand their state to the lower ones, these are merged by rows
+    PagedCursor following = c;
+    const bool done = x + count >= x_end;
+    if (!done) {
+      paged_next_stream(a, following);
+      if constexpr (QREG) load_q(following);  // arrives during the merge
+    }
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], d);
-        if (l4 == 0) ml_s[warp * ROWS + 8 * nb + 2 * t4 + j] = make_float2(m[nb][j], l[nb][j]);
+    auto put = [&](int entry) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          if (l4 == 0) ml_s[entry * ROWS + 8 * nb + 2 * t4 + j] = make_float2(m[nb][j], l[nb][j]);
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc_s[merge_at(entry, 8 * nb + 2 * t4 + (j & 1), ROWS, db * 16 + l4 + (j >> 1) * 8)] = o[nb][db][j];
       }
+    };
+    __syncthreads();  // the merge buffer (and q_s) of the stream before has been read
+    if (warp >= kHalf) put(warp - kHalf);
+    __syncthreads();
+    if (warp < kHalf) {
 #pragma unroll
-      for (int db = 0; db < 8; ++db)
+      for (int nb = 0; nb < NB; ++nb) {
+        float f[2], g[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc_s[((size_t)warp * ROWS + 8 * nb + 2 * t4 + (j & 1)) * kAccStride + db * 16 + l4 + (j >> 1) * 8] = o[nb][db][j];
+        for (int j = 0; j < 2; ++j) {
+          const float2 other = ml_s[warp * ROWS + 8 * nb + 2 * t4 + j];
+          const float to = fmaxf(m[nb][j], other.x);
+          f[j] = ex2(m[nb][j] - to);
+          g[j] = ex2(other.x - to);
+          m[nb][j] = to;
+          l[nb][j] = fmaf(l[nb][j], f[j], other.y * g[j]);
+        }
+#pragma unroll
+        for (int db = 0; db < 8; ++db)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[nb][db][j] = fmaf(o[nb][db][j], f[j & 1], g[j & 1] * acc_s[merge_at(warp, 8 * nb + 2 * t4 + (j & 1), ROWS, db * 16 + l4 + (j >> 1) * 8)]);
+      }
+      __syncwarp();
+      put(warp);
     }
     __syncthreads();
-    paged_finish<E>(a, c, x - c.tile, c.tile, count, total, C, rows, ROWS, ml_s, acc_s, &last_s);
+    paged_finish<E, ROWS>(a, sh, c, x, count, rows, kHalf, ml_s, acc_s, pend_s);
+    if (done) break;
+    if constexpr (!QREG) load_q(following);  // q_s was last read before the merge
     x += count;
-    if (x >= x_end) return;
-    __syncthreads();  // the rings are free again
-    paged_next_stream(a, c);
+    c = following;
   }
+  cp_async_wait<0>();
+  paged_fold<E, ROWS>(a, pend_s, ml_s, acc_s);
 }
 
-template <typename E, int NB, int STAGES>
+template <typename E, int NB, int STAGES, bool SHAPED>
 static int launch_mma(const PagedArgs& a, cudaStream_t st) {
   constexpr int ROWS = 8 * NB;
-  constexpr size_t ring = (size_t)kPWarps * STAGES * 2 * kMKeys * kD * 2;
-  constexpr size_t merge = sizeof(float) * kPWarps * ROWS * kAccStride;
-  constexpr size_t smem = (ring > merge ? ring : merge) + sizeof(float2) * kPWarps * ROWS + (NB > 2 ? ROWS * 256 : 0);
-  static_assert(smem <= 220 * 1024, "shared memory of a CTA");
-  auto kern = paged_attend_mma_kernel<E, NB, STAGES>;
+  constexpr size_t smem = (size_t)kPWarps * STAGES * 2 * kMKeys * kD * 2 + sizeof(float) * (kPWarps / 2) * ROWS * kD +
+                          sizeof(float2) * kPWarps * ROWS + (NB > 2 ? ROWS * 256 : 0);
+  static_assert(smem <= 225 * 1024 + 512, "shared memory of a CTA");
+  auto kern = paged_attend_mma_kernel<E, NB, STAGES, SHAPED>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return check_launch("paged_attend shared memory");
   kern<<<sm_count(), kPThreads, smem, st>>>(a);
@@ -721,28 +847,46 @@ static int launch_mma(const PagedArgs& a, cudaStream_t st) {
 
 // ---- accumulated weights -----------------------------------------------------------------------------
 // mass[r, h, i] += sum over the rows of 2^(s - lse): one pass over the scores the attention kernel left (4 bytes per
-// row and key, which come from L2 while the cache rows went past it), the same shares of the same tiles.  The rows of
-// a key are added in row order by one thread: no atomics, the same bits every run.
-__global__ void __launch_bounds__(256) paged_mass_kernel(const PagedArgs a) {
-  const long long total = paged_total(a);  // a.groups is 1 here: one stream per KV head
-  long long x = paged_share(total, blockIdx.x, gridDim.x);
-  const long long x_end = paged_share(total, blockIdx.x + 1, gridDim.x);
-  if (x >= x_end) return;
-  PagedCursor c = paged_locate(a, x);
-  const int keys = 1 << a.tile_log2;
+// row and key, which come from L2 while the cache rows went past it), the same tiles in equal shares, four keys to a
+// thread.  The rows of a key are added in row order by one thread: no atomics, the same bits every run.
+constexpr int kMassThreads = 128;
+__global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArgs a) {
+  // a.groups is 1 here: one stream per KV head
+  PagedCursor c;
+  const PagedShares sh = paged_locate(a, gridDim.x, blockIdx.x, c);
+  if (blockIdx.x >= sh.C) return;
+  int x = sh.first(blockIdx.x);
+  const int x_end = sh.first(blockIdx.x + 1);
+  const int quads = a.tile_log2 - 2;  // log2 of the quads of keys in a tile
+  dependents_wait();  // what the attention kernel wrote is needed from here on
   while (true) {
-    const int count = (int)min((long long)(c.g.tiles - c.tile), x_end - x);
-    const int64_t stream = (int64_t)c.r * a.H + c.sub;
-    for (int i = threadIdx.x; i < count * keys; i += blockDim.x) {
-      const int slot = paged_tile(c.g, c.tile + (i >> a.tile_log2)) * keys + (i & (keys - 1));
+    const int count = min(c.g.tiles - c.tile, x_end - x);
+    const int64_t stream = (int64_t)c.r * a.H + c.h;
+    for (int i = threadIdx.x; i < count << quads; i += kMassThreads) {
+      const int slot = (paged_tile(c.g, c.tile + (i >> quads)) << a.tile_log2) + ((i & ((1 << quads) - 1)) << 2);
       if (slot >= c.g.n) continue;
-      float w = 0.f;
-      for (int row = 0; row < a.R; ++row) {
-        const float s = __ldcg(a.scores + (stream * a.R + row) * a.cap + slot);
-        const float z = __ldcg(a.row_lse2 + stream * a.R + row);
-        w += s == kNegInf ? 0.f : ex2(s - z);
+      float w[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int row0 = 0; row0 < a.R; row0 += 4) {
+        float4 s[4];
+        float z[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = min(row0 + j, a.R - 1);
+          s[j] = __ldcg(reinterpret_cast<const float4*>(a.scores + (stream * a.R + row) * a.score_stride + slot));
+          z[j] = row0 + j < a.R ? __ldcg(a.row_lse2 + stream * a.R + row) : -kNegInf;  // 2^(s - inf) = 0: a row that is not there
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[0] += s[j].x == kNegInf ? 0.f : ex2(s[j].x - z[j]);
+          w[1] += s[j].y == kNegInf ? 0.f : ex2(s[j].y - z[j]);
+          w[2] += s[j].z == kNegInf ? 0.f : ex2(s[j].z - z[j]);
+          w[3] += s[j].w == kNegInf ? 0.f : ex2(s[j].w - z[j]);
+        }
       }
-      if (w != 0.f) a.mass[stream * a.cap + slot] += w;  // keys no row saw are left as they were
+      float* to = a.mass + stream * a.cap + slot;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (slot + j < c.g.n && w[j] != 0.f) to[j] += w[j];  // keys no row saw are left as they were
     }
     x += count;
     if (x >= x_end) return;
@@ -753,8 +897,21 @@ __global__ void __launch_bounds__(256) paged_mass_kernel(const PagedArgs a) {
 int launch_paged_mass(const PagedArgs& a, cudaStream_t st) {
   PagedArgs b = a;
   b.groups = 1;
-  paged_mass_kernel<<<sm_count() * 8, 256, 0, st>>>(b);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sm_count() * 8);
+  cfg.blockDim = dim3(kMassThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, paged_mass_kernel, b) != cudaSuccess) return check_launch("paged_mass");
   return check_launch("paged_mass");
+}
+
+template <typename E, bool SHAPED> static int launch_16bit(const PagedArgs& a, int rows, cudaStream_t st) {
+  return rows <= 8 ? launch_mma<E, 1, 3, SHAPED>(a, st) : rows <= 16 ? launch_mma<E, 2, 3, SHAPED>(a, st) : launch_mma<E, 4, 2, SHAPED>(a, st);
 }
 
 int launch_paged_attend(const PagedArgs& a, int dtype, cudaStream_t st) {
@@ -763,16 +920,14 @@ int launch_paged_attend(const PagedArgs& a, int dtype, cudaStream_t st) {
   int rc = PQHSA_OK;
   if (dtype == PQHSA_F32) {
     b.tile_log2 = 3;
-    rc = rows <= 8 ? launch_simple<float, 8, 2>(b, st) : rows <= 16 ? launch_simple<float, 16, 2>(b, st) : launch_simple<float, 32, 2>(b, st);
+    rc = rows <= 4 ? launch_fp32<4, 3>(b, st) : rows <= 8 ? launch_fp32<8, 3>(b, st) : rows <= 16 ? launch_fp32<16, 3>(b, st) : launch_fp32<32, 3>(b, st);
   } else {
     b.tile_log2 = 4;
-    if (dtype == PQHSA_BF16) {
-      using E = __nv_bfloat16;
-      rc = rows <= 8 ? launch_mma<E, 1, 3>(b, st) : rows <= 16 ? launch_mma<E, 2, 3>(b, st) : launch_mma<E, 4, 3>(b, st);
-    } else {
-      using E = __half;
-      rc = rows <= 8 ? launch_mma<E, 1, 3>(b, st) : rows <= 16 ? launch_mma<E, 2, 3>(b, st) : launch_mma<E, 4, 3>(b, st);
-    }
+    const bool shaped = a.softcap > 0.f || a.slopes != nullptr;
+    if (dtype == PQHSA_BF16)
+      rc = shaped ? launch_16bit<__nv_bfloat16, true>(b, rows, st) : launch_16bit<__nv_bfloat16, false>(b, rows, st);
+    else
+      rc = shaped ? launch_16bit<__half, true>(b, rows, st) : launch_16bit<__half, false>(b, rows, st);
   }
   if (rc != PQHSA_OK || a.mass == nullptr) return rc;
   return launch_paged_mass(b, st);

@@ -34,7 +34,7 @@ ATTENTION = [
     ({"requests": -1}, -2, "requests"), ({"requests": 70000}, -2, "requests"), ({"kv_heads": 0}, -2, "kv_heads"),
     ({"group": 0}, -2, "group"), ({"group": 17}, -2, "group"), ({"query_len": 0}, -2, "query_len"), ({"query_len": 9}, -2, "query_len"),
     ({"group": 16, "query_len": 5}, -2, "group * query_len"), ({"slot_capacity": 0}, -2, "slot_capacity"),
-    ({"slot_capacity": (1 << 24) + 1}, -2, "slot_capacity"), ({"kv_heads": 1024, "slot_capacity": 1 << 24}, -2, "too large"),
+    ({"slot_capacity": (1 << 24) + 1}, -2, "slot_capacity"), ({"kv_heads": 1024, "slot_capacity": 1 << 24}, -2, "2^33"),
     ({"k_base": None}, -1, "k_base"), ({"seq_lens": None}, -1, "seq_lens"), ({"block_size": 0}, -2, "block_size"),
     ({"num_blocks": 0}, -2, "num_blocks"), ({"max_blocks": 0}, -2, "max_blocks"), ({"block_table": None, "num_blocks": 1}, -2, "contiguous"),
     ({"stride_row": 127}, -2, "aligned"), ({"k_base": A + 2}, -2, "aligned"), ({"window": -1}, -2, "window"),
