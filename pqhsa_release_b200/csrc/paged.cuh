@@ -2,6 +2,8 @@
 // a request are visible, and how the key tiles of all requests are shared out over a persistent grid.
 #pragma once
 
+#include <utility>
+
 #include "common.cuh"
 
 namespace pqhsa {
@@ -59,9 +61,31 @@ int launch_paged_append(const PagedArgs& a, const void* k, const void* v, int32_
 
 #ifdef __CUDACC__
 
-// A kernel launched with programmatic stream serialization starts while the one before it ends; from here on it sees
-// all that one wrote.
-__device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Launch with the attributes of the paged kernels; cluster > 0: as clusters of that many CTAs in x.
+template <typename... P, typename... A>
+static inline cudaError_t paged_launch(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, A&&... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<A>(args)...);
+}
+
+// Every kernel here is launched with programmatic stream serialization: it may be placed on the GPU while the one
+// before it in the stream ends.  wait_for_grid comes before its first access to global memory: from there on it sees
+// all that came before.  next_grid lets the kernel behind be placed from now on instead of at this one's end.
+__device__ __forceinline__ void wait_for_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void next_grid() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // Element offset of slot t of request r, KV head h; negative when the slot's page is not in the cache (a block-table
 // entry outside 0 .. num_blocks - 1: such a key is invisible, nothing of it is read or written).

@@ -89,13 +89,13 @@ struct PagedPending {
 
 // Ends a stream in this share (all threads): the states of `entries` warps in ml [entries][ROWS] and acc are merged and
 // written as output rows (the share holds the whole stream) or as a part of it.
-template <typename E, int ROWS>
+template <typename E, int ROWS, int WARPS>
 __device__ __forceinline__ void paged_finish(const PagedArgs& a, const PagedShares& sh, const PagedCursor& c, int x, int count,
                                              int rows, int entries, const float2* ml, const float* acc, PagedPending* pend) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool starts = c.tile == 0, whole = starts && count == c.g.tiles;
   const size_t part = (size_t)2 * blockIdx.x + (starts ? 1 : 0);
-  for (int row = warp; row < rows; row += kPWarps) {
+  for (int row = warp; row < rows; row += WARPS) {
     RowSum s;
     for (int w = 0; w < entries; ++w) s.M = fmaxf(s.M, ml[w * ROWS + row].x);
     for (int w = 0; w < entries; ++w)
@@ -117,74 +117,86 @@ __device__ __forceinline__ void paged_finish(const PagedArgs& a, const PagedShar
   }
 }
 
-// After the last tile of the CTA (all threads): tickets for its parts, and the fold of the streams it ends.
-template <typename E, int ROWS>
-__device__ __forceinline__ void paged_fold(const PagedArgs& a, PagedPending* pend, float2* ml, float* acc) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  __syncthreads();  // the parts are written (by all threads) and pend is set
-  if (threadIdx.x == 0) {
-    if ((pend[0].parts | pend[1].parts) != 0) __threadfence();
+// Folds every `by`-th part of a row of stream p from part `at` on (a warp; eight parts' loads in flight).
+template <int ROWS>
+__device__ __forceinline__ RowSum paged_fold_row(const PagedArgs& a, const PagedPending& p, int row, int at, int by) {
+  constexpr int kAhead = 8;
+  const int lane = threadIdx.x & 31;
+  RowSum s;
+  for (int p0 = at; p0 < p.parts; p0 += kAhead * by) {
+    float2 x[kAhead];
+    float4 v[kAhead];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      pend[i].last = 0;
-      if (pend[i].parts == 0) continue;
-      if (atomicAdd(a.tickets + pend[i].c0, 1) == pend[i].parts - 1) {
-        pend[i].last = 1;
-        a.tickets[pend[i].c0] = 0;
+    for (int u = 0; u < kAhead; ++u) {
+      const int q = p0 + u * by;
+      x[u] = make_float2(kFloor, 0.f);
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (q < p.parts) {
+        const size_t place = (size_t)2 * (p.c0 + q) + (q == 0 ? 1 : 0);
+        x[u] = __ldcg(&a.part_ml[place * kPagedGroupRows + row]);
+        v[u] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + (place * ROWS + row) * kD + lane * 4));
       }
     }
+    float top = x[0].x;
+#pragma unroll
+    for (int u = 1; u < kAhead; ++u) top = fmaxf(top, x[u].x);
+    s.raise(top);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) s.add(x[u], v[u]);
+  }
+  return s;
+}
+
+// After the last tile of the CTA (all threads): tickets for its parts, and the fold of the streams it ends.
+template <typename E, int ROWS, int WARPS>
+__device__ __forceinline__ void paged_fold(const PagedArgs& a, PagedPending* pend, float2* ml, float* acc) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  next_grid();
+  __syncthreads();  // the parts are written (by all threads) and pend is set
+  if (threadIdx.x < 2 && pend[threadIdx.x].parts != 0) {
+    PagedPending& p = pend[threadIdx.x];
     __threadfence();
+    p.last = atomicAdd(a.tickets + p.c0, 1) == p.parts - 1;
+    if (p.last != 0) {
+      a.tickets[p.c0] = 0;
+      __threadfence();
+    }
   }
   __syncthreads();
+  // rows of both streams, a warp each, while the parts of a row are few
+  constexpr int kFew = 16;
+  const auto rows_of = [&](int i) { return pend[i].last != 0 ? min(a.R - pend[i].pass * kPagedGroupRows, kPagedGroupRows) : 0; };
+  const int rows0 = pend[0].parts <= kFew ? rows_of(0) : 0, rows1 = pend[1].parts <= kFew ? rows_of(1) : 0;
+  for (int item = warp; item < rows0 + rows1; item += WARPS) {
+    const PagedPending& p = pend[item < rows0 ? 0 : 1];
+    const int row = item < rows0 ? item : item - rows0;
+    const RowSum s = paged_fold_row<ROWS>(a, p, row, 0, 1);
+    paged_store_row<E>(a, p.r, p.h, p.pass, row, lane, s.M, s.L, s.o);
+  }
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
-    if (pend[i].last == 0) continue;
-    const int parts = pend[i].parts, c0 = pend[i].c0, rows = min(a.R - pend[i].pass * kPagedGroupRows, kPagedGroupRows);
-    // warps of a row: all of them for one row, one for eight and more; each folds every per-th part
-    const int per = rows <= 1 ? kPWarps : rows <= 2 ? kPWarps / 2 : rows <= 4 ? kPWarps / 4 : 1;
+    const PagedPending& p = pend[i];
+    const int rows = p.parts > kFew ? rows_of(i) : 0;
+    // a long stream: several warps to a row (all of them for one row, one for eight), each folds every per-th part
+    const int per = rows <= 1 ? WARPS : rows <= 2 ? WARPS / 2 : rows <= 4 ? WARPS / 4 : 1;
     const int at = warp % per;
-    for (int base = 0; base < rows; base += kPWarps / per) {
+    for (int base = 0; base < rows; base += WARPS / per) {
       const int row = base + warp / per;
       RowSum s;
-      if (row < rows) {
-        constexpr int kAhead = 8;  // loads in flight
-        for (int p0 = at; p0 < parts; p0 += kAhead * per) {
-          float2 x[kAhead];
-          float4 v[kAhead];
-#pragma unroll
-          for (int u = 0; u < kAhead; ++u) {
-            const int p = p0 + u * per;
-            const size_t place = (size_t)2 * (c0 + min(p, parts - 1)) + (min(p, parts - 1) == 0 ? 1 : 0);
-            x[u] = __ldcg(&a.part_ml[place * kPagedGroupRows + row]);
-            v[u] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + (place * ROWS + row) * kD + lane * 4));
-            if (p >= parts) {
-              x[u] = make_float2(kFloor, 0.f);
-              v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-          }
-          float top = x[0].x;
-#pragma unroll
-          for (int u = 1; u < kAhead; ++u) top = fmaxf(top, x[u].x);
-          s.raise(top);
-#pragma unroll
-          for (int u = 0; u < kAhead; ++u) s.add(x[u], v[u]);
-        }
-        if (per == 1) paged_store_row<E>(a, pend[i].r, pend[i].h, pend[i].pass, row, lane, s.M, s.L, s.o);
-      }
-      if (per == 1) continue;
-      __syncthreads();  // the buffer of the round before has been read
-      if (lane == 0) ml[warp] = make_float2(s.M, s.L);
-      *reinterpret_cast<float4*>(acc + warp * kD + lane * 4) = s.o;
-      __syncthreads();
-      if (at == 0 && row < rows) {
+      if (row < rows) s = paged_fold_row<ROWS>(a, p, row, at, per);
+      if (per > 1) {
+        __syncthreads();  // the buffer of the round before has been read
+        if (lane == 0) ml[warp] = make_float2(s.M, s.L);
+        *reinterpret_cast<float4*>(acc + warp * kD + lane * 4) = s.o;
+        __syncthreads();
+        if (at != 0) continue;
         for (int w = warp + 1; w < warp + per; ++w) {
           s.raise(ml[w].x);
           s.add(ml[w], *reinterpret_cast<const float4*>(acc + w * kD + lane * 4));
         }
-        paged_store_row<E>(a, pend[i].r, pend[i].h, pend[i].pass, row, lane, s.M, s.L, s.o);
       }
+      if (row < rows) paged_store_row<E>(a, p.r, p.h, p.pass, row, lane, s.M, s.L, s.o);
     }
-    __syncthreads();
   }
 }
 
@@ -197,19 +209,19 @@ __device__ __forceinline__ float4 tile_piece(const float* tile, int key, int ele
   return *reinterpret_cast<const float4*>(tile + key * kD + (((elem >> 2) ^ (key & 7)) << 2));
 }
 
-template <int ROWS, int STAGES>
-__global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedArgs a) {
+template <int ROWS, int STAGES, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const PagedArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr int kStage = 2 * kKeys * kD;  // elements of a stage: 8 key rows, then 8 value rows
   constexpr int OWN = ROWS / 4;
   float* ring = reinterpret_cast<float*>(smem_raw) + (threadIdx.x >> 5) * (STAGES * kStage);
   float* acc_s = reinterpret_cast<float*>(smem_raw);  // merge buffer over the rings, used between streams
   static_assert(ROWS <= 2 * STAGES * kKeys, "the merge buffer fits the rings");
-  float* q_s = reinterpret_cast<float*>(smem_raw) + kPWarps * STAGES * kStage;         // [ROWS][128]
+  float* q_s = reinterpret_cast<float*>(smem_raw) + WARPS * STAGES * kStage;         // [ROWS][128]
   float* p_s = q_s + ROWS * kD + (threadIdx.x >> 5) * (ROWS * kKeys);                  // per warp [ROWS][8]
-  float2* ml_s = reinterpret_cast<float2*>(q_s + ROWS * kD + kPWarps * ROWS * kKeys);  // [warps][ROWS]
-  __shared__ int pos_s[kPWarps][STAGES][kKeys];
-  __shared__ int seen_s[kPWarps][STAGES];  // keys some row of the step sees; << 16: keys not all of them see
+  float2* ml_s = reinterpret_cast<float2*>(q_s + ROWS * kD + WARPS * ROWS * kKeys);  // [warps][ROWS]
+  __shared__ int pos_s[WARPS][STAGES][kKeys];
+  __shared__ int seen_s[WARPS][STAGES];  // keys some row of the step sees; << 16: keys not all of them see
   __shared__ PagedPending pend_s[2];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -217,22 +229,23 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
   const float* kb = static_cast<const float*>(a.k_base);
   const float* vb = static_cast<const float*>(a.v_base);
 
+  if (tid < 2) pend_s[tid].parts = pend_s[tid].last = 0;
+  wait_for_grid();
   PagedCursor c;
   const PagedShares sh = paged_locate(a, gridDim.x, blockIdx.x, c);
   if (blockIdx.x >= sh.C) return;
   int x = sh.first(blockIdx.x);
   const int x_end = sh.first(blockIdx.x + 1);
-  if (tid < 2) pend_s[tid].parts = 0;
 
   while (true) {
     const int count = min(c.g.tiles - c.tile, x_end - x);  // tiles of this stream in the share
     const int h = c.h, row0 = c.pass * kPagedGroupRows, rows = min(a.R - row0, kPagedGroupRows);
-    const int mine = count > warp ? (count - warp + kPWarps - 1) / kPWarps : 0;
+    const int mine = count > warp ? (count - warp + WARPS - 1) / WARPS : 0;
     const int32_t* kpos = a.key_pos != nullptr ? a.key_pos + ((int64_t)c.r * a.H + h) * a.cap : nullptr;
     // fills ring slot `st` with tile number `it` of this warp
     auto load = [&](int it, int st) {
       if (it < mine) {
-        const int slot = paged_tile(c.g, c.tile + warp + it * kPWarps) * kKeys + key;
+        const int slot = paged_tile(c.g, c.tile + warp + it * WARPS) * kKeys + key;
         int64_t off = -1;
         int pos = -1;
         if (slot < c.g.n) {
@@ -259,7 +272,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
     __syncthreads();  // the merge buffer and q_s are free again
 #pragma unroll
     for (int st = 0; st < STAGES - 1; ++st) load(st, st);
-    for (int i = tid; i < ROWS * (kD / 4); i += kPThreads) {
+    for (int i = tid; i < ROWS * (kD / 4); i += WARPS * 32) {
       const int row = i / (kD / 4), d = i % (kD / 4) * 4, full = row0 + row;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < rows)
@@ -321,7 +334,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
         raise |= own[i] > m[i] + kLazy;
       }
       if (a.scores != nullptr) {
-        const int slot = paged_tile(c.g, c.tile + warp + it * kPWarps) * kKeys + key;
+        const int slot = paged_tile(c.g, c.tile + warp + it * WARPS) * kKeys + key;
         float* dst = a.scores + (((int64_t)c.r * a.H + h) * a.R + row0) * a.score_stride + slot;
         if (slot < c.g.n) {
 #pragma unroll
@@ -389,24 +402,24 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_kernel(const PagedA
     for (int i = 0; i < ROWS; ++i)
       *reinterpret_cast<float4*>(acc_s + merge_at(warp, i, ROWS, lane * 4)) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
     __syncthreads();
-    paged_finish<float, ROWS>(a, sh, c, x, count, rows, kPWarps, ml_s, acc_s, pend_s);
+    paged_finish<float, ROWS, WARPS>(a, sh, c, x, count, rows, WARPS, ml_s, acc_s, pend_s);
     x += count;
     if (x >= x_end) break;
     paged_next_stream(a, c);
   }
-  paged_fold<float, ROWS>(a, pend_s, ml_s, acc_s);
+  paged_fold<float, ROWS, WARPS>(a, pend_s, ml_s, acc_s);
 }
 
-template <int ROWS, int STAGES>
+template <int ROWS, int STAGES, int WARPS>
 static int launch_fp32(const PagedArgs& a, cudaStream_t st) {
-  constexpr size_t smem = sizeof(float) * (kPWarps * STAGES * 2 * kKeys * kD + ROWS * kD + kPWarps * ROWS * kKeys) +
-                          sizeof(float2) * kPWarps * ROWS;
+  constexpr size_t smem = sizeof(float) * (WARPS * STAGES * 2 * kKeys * kD + ROWS * kD + WARPS * ROWS * kKeys) +
+                          sizeof(float2) * WARPS * ROWS;
   static_assert(smem <= 225 * 1024, "shared memory of a CTA");
-  auto kern = paged_attend_kernel<ROWS, STAGES>;
+  auto kern = paged_attend_kernel<ROWS, STAGES, WARPS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return check_launch("paged_attend shared memory");
-  kern<<<sm_count(), kPThreads, smem, st>>>(a);
-  return check_launch("paged_attend");
+  if (paged_launch(kern, dim3(sm_count()), WARPS * 32, smem, st, 0, a) != cudaSuccess) return check_launch("paged_attend");
+  return PQHSA_OK;
 }
 
 // ---- tensor-core kernel for 16-bit caches: tiles of 16 keys ----------------------------------------------
@@ -485,12 +498,13 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
   const int g_row = lane >> 3, g_piece = lane & 7;                                              // copies: 4 rows x 128 bytes at a time
   const uint32_t g_lane = ring + g_row * 256 + ((g_piece ^ g_row) << 4);
 
+  if (tid < 2) pend_s[tid].parts = pend_s[tid].last = 0;
+  wait_for_grid();
   PagedCursor c;
   const PagedShares sh = paged_locate(a, gridDim.x, blockIdx.x, c);
   if (blockIdx.x >= sh.C) return;
   int x = sh.first(blockIdx.x);
   const int x_end = sh.first(blockIdx.x + 1);
-  if (tid < 2) pend_s[tid].parts = 0;
 
   // the copies' cursor: tile number `at` of the `at_end` of this warp in stream `ahead`
   PagedCursor ahead = c;
@@ -822,14 +836,14 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
       put(warp);
     }
     __syncthreads();
-    paged_finish<E, ROWS>(a, sh, c, x, count, rows, kHalf, ml_s, acc_s, pend_s);
+    paged_finish<E, ROWS, kPWarps>(a, sh, c, x, count, rows, kHalf, ml_s, acc_s, pend_s);
     if (done) break;
     if constexpr (!QREG) load_q(following);  // q_s was last read before the merge
     x += count;
     c = following;
   }
   cp_async_wait<0>();
-  paged_fold<E, ROWS>(a, pend_s, ml_s, acc_s);
+  paged_fold<E, ROWS, kPWarps>(a, pend_s, ml_s, acc_s);
 }
 
 template <typename E, int NB, int STAGES, bool SHAPED>
@@ -841,8 +855,8 @@ static int launch_mma(const PagedArgs& a, cudaStream_t st) {
   auto kern = paged_attend_mma_kernel<E, NB, STAGES, SHAPED>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return check_launch("paged_attend shared memory");
-  kern<<<sm_count(), kPThreads, smem, st>>>(a);
-  return check_launch("paged_attend");
+  if (paged_launch(kern, dim3(sm_count()), kPThreads, smem, st, 0, a) != cudaSuccess) return check_launch("paged_attend");
+  return PQHSA_OK;
 }
 
 // ---- accumulated weights -----------------------------------------------------------------------------
@@ -858,7 +872,7 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArg
   int x = sh.first(blockIdx.x);
   const int x_end = sh.first(blockIdx.x + 1);
   const int quads = a.tile_log2 - 2;  // log2 of the quads of keys in a tile
-  dependents_wait();  // what the attention kernel wrote is needed from here on
+  wait_for_grid();  // scores and row sums are there
   while (true) {
     const int count = min(c.g.tiles - c.tile, x_end - x);
     const int64_t stream = (int64_t)c.r * a.H + c.h;
@@ -897,17 +911,8 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArg
 int launch_paged_mass(const PagedArgs& a, cudaStream_t st) {
   PagedArgs b = a;
   b.groups = 1;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(sm_count() * 8);
-  cfg.blockDim = dim3(kMassThreads);
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, paged_mass_kernel, b) != cudaSuccess) return check_launch("paged_mass");
-  return check_launch("paged_mass");
+  if (paged_launch(paged_mass_kernel, dim3(sm_count() * 8), kMassThreads, 0, st, 0, b) != cudaSuccess) return check_launch("paged_mass");
+  return PQHSA_OK;
 }
 
 template <typename E, bool SHAPED> static int launch_16bit(const PagedArgs& a, int rows, cudaStream_t st) {
@@ -920,7 +925,7 @@ int launch_paged_attend(const PagedArgs& a, int dtype, cudaStream_t st) {
   int rc = PQHSA_OK;
   if (dtype == PQHSA_F32) {
     b.tile_log2 = 3;
-    rc = rows <= 4 ? launch_fp32<4, 3>(b, st) : rows <= 8 ? launch_fp32<8, 3>(b, st) : rows <= 16 ? launch_fp32<16, 3>(b, st) : launch_fp32<32, 3>(b, st);
+    rc = rows <= 4 ? launch_fp32<4, 2, 12>(b, st) : rows <= 8 ? launch_fp32<8, 2, 12>(b, st) : rows <= 16 ? launch_fp32<16, 3, 8>(b, st) : launch_fp32<32, 3, 8>(b, st);
   } else {
     b.tile_log2 = 4;
     const bool shaped = a.softcap > 0.f || a.slopes != nullptr;

@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
   };
   const int64_t stream = blockIdx.y;
   const int r = blockIdx.y / a.H;
+  wait_for_grid();
   const int n = min(max(__ldg(a.seq_lens + r), 0), a.limit), K = e.budget;
   const float* mass = a.mass + stream * a.cap;
   const int32_t* pos = a.key_pos + stream * a.cap;
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(const PagedArgs a, c
   E* vb = static_cast<E*>(const_cast<void*>(a.v_base));
   constexpr int half = sizeof(E) / 2;  // 16-byte pieces of a row for each of 16 lanes
   long long w = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  dependents_wait();  // launched while the selection ends
+  wait_for_grid();
   int dst = -1, src = -1;
   auto fetch = [&](long long item) {
     dst = -1;
@@ -414,30 +415,13 @@ int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaS
   auto kern = resident ? evict_select_kernel<true> : evict_select_kernel<false>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return check_launch("evict_select shared memory");
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ranks;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ranks, a.B * a.H);
-  cfg.blockDim = dim3(kEvThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, a, e) != cudaSuccess) return check_launch("evict_select");
+  if (paged_launch(kern, dim3(ranks, a.B * a.H), kEvThreads, smem, st, ranks, a, e) != cudaSuccess) return check_launch("evict_select");
   const int most = e.budget < a.limit ? (e.budget < a.limit - e.budget ? e.budget : a.limit - e.budget) : 0;
   const int per = (most + kEvMoves - 1) / kEvMoves;
   const long long want = ((long long)a.B * a.H * per + 7) / 8 + 1, cap = (long long)sm_count() * 4;
   const unsigned grid = (unsigned)(want < cap ? want : cap);
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
   PQHSA_DISPATCH_E(dtype, {
-    if (cudaLaunchKernelEx(&cfg, evict_move_kernel<E>, a, e, per > 0 ? per : 1) != cudaSuccess) return check_launch("evict_move");
+    if (paged_launch(evict_move_kernel<E>, dim3(grid), 256, 0, st, 0, a, e, per > 0 ? per : 1) != cudaSuccess) return check_launch("evict_move");
   });
   return check_launch("evict_move");
 }
@@ -449,6 +433,7 @@ template <typename E>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedArgs a, const E* __restrict__ k, const E* __restrict__ v,
                                                            int32_t* new_lens) {
   const int r = blockIdx.x, lane = threadIdx.x & 31;
+  wait_for_grid();
   const int n = a.seq_lens[r];
   E* kb = static_cast<E*>(const_cast<void*>(a.k_base));
   E* vb = static_cast<E*>(const_cast<void*>(a.v_base));
@@ -474,8 +459,10 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedArgs a, co
 }
 
 int launch_paged_append(const PagedArgs& a, const void* k, const void* v, int32_t* new_lens, int dtype, cudaStream_t st) {
-  PQHSA_DISPATCH_E(dtype, (paged_append_kernel<E><<<a.B, 256, 0, st>>>(a, static_cast<const E*>(k), static_cast<const E*>(v),
-                                                                      new_lens)));
+  PQHSA_DISPATCH_E(dtype, {
+    if (paged_launch(paged_append_kernel<E>, dim3(a.B), 256, 0, st, 0, a, static_cast<const E*>(k), static_cast<const E*>(v), new_lens) != cudaSuccess)
+      return check_launch("paged_append");
+  });
   return check_launch("paged_append");
 }
 
