@@ -2,6 +2,7 @@
 // a request are visible, and how the key tiles of all requests are shared out over a persistent grid.
 #pragma once
 
+#include <atomic>
 #include <utility>
 
 #include "common.cuh"
@@ -42,7 +43,13 @@ struct PagedArgs {
   float* row_lse2;             // [B * H][R] log2 sum 2^s of every query row
   float* scores;               // [B * H][R][score_stride] scores in log2 units, only with mass
   int64_t score_stride;        // cap, rounded up to whole tiles
+  int32_t g_inv;               // 65536 / G + 1: row / G of the few rows there are without a division
   int32_t tile_log2;           // keys per tile of the attention kernel that runs (fixes the shares)
+
+  // token, query head in the group and place of query row `row` (token * G + head) of a KV head
+  __host__ __device__ int token_of(int row) const { return row * g_inv >> 16; }
+  __host__ __device__ int head_of(int row) const { return row - token_of(row) * G; }
+  __host__ __device__ int64_t q_row(int row) const { return token_of(row) * q_st + head_of(row) * q_sh; }
 };
 
 int launch_paged_attend(const PagedArgs& a, int dtype, cudaStream_t st);
@@ -60,6 +67,17 @@ int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaS
 int launch_paged_append(const PagedArgs& a, const void* k, const void* v, int32_t* new_lens, int dtype, cudaStream_t st);
 
 #ifdef __CUDACC__
+
+// Lets a kernel have `smem` bytes of dynamic shared memory on the current device (asked of the runtime once a device).
+static inline cudaError_t paged_allow_smem(const void* kern, size_t smem, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev); e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Launch with the attributes of the paged kernels; cluster > 0: as clusters of that many CTAs in x.
 template <typename... P, typename... A>
@@ -154,25 +172,30 @@ __device__ __forceinline__ PagedSight paged_sight(const PagedGeom& g, const Page
   return s;
 }
 
-// The tiles of all streams - stream (r, h, pass) in that order - form one sequence of `total` (the host refuses shapes
-// that could pass 31 bits), of which each of C CTAs takes a contiguous share: total / C tiles, one more for the first
-// total % C of them.  Equal shares whatever the lengths; every warp finds its CTA's by itself.
+// How the key tiles of all streams - stream (r, h, pass) in that order, `total` tiles (the host refuses shapes that
+// could pass 31 bits) - are shared out over the CTAs, whatever the lengths; every warp works it out by itself.
+//
+// Equal shares: the tiles form one sequence of which each of C CTAs takes a contiguous share, total / C tiles, one more
+// for the first total % C of them.  No CTA has more to do than another, but one whose share runs over the end of a
+// stream pays for the merge and the start twice.
+//
+// Aligned shares, with no more streams than CTAs: every stream gets CTAs of its own, in proportion to its tiles and no
+// more than give each warp a tile.  Taken where the largest share is at most half as large again as an equal one and
+// kPagedSlack tiles more: a second stream costs a CTA about 2 us, the time of some 12 tiles of 8 KB at an SM's part of
+// the memory rate, and an SM that has more to read than others can draw more than its part of it.  us, aligned against
+// equal, with the largest share over the equal one (8 KV heads): one request of 1K 9.3 / 13.9 (2.3, slack); 16 of 4096
+// 48.1 / 50.1 (1.2); a 4-token step of 8 requests in windows of 4096 34.3 / 37.4 (1.5); 9 of 2K-12K 60.0 / 49.5 (1.95).
+constexpr int kPagedSlack = 12;
 struct PagedShares {
   int total, C, q, rem;
+  int c0, parts;    // aligned: first CTA of this CTA's stream, and how many it has; else parts = 0
+  int x, x_end;     // tiles of this CTA, counted along the sequence (equal shares) or in its stream (aligned)
   __device__ __forceinline__ int first(int c) const { return c * q + min(c, rem); }
-  __device__ __forceinline__ int owner(int x) const {  // CTA that has tile x
+  __device__ __forceinline__ int owner(int x) const {  // equal shares: CTA that has tile x
     const int wide = rem * (q + 1);
     return x < wide ? x / (q + 1) : rem + (x - wide) / q;
   }
 };
-__device__ __forceinline__ PagedShares paged_shares(int total, int ctas) {
-  PagedShares s;
-  s.total = total;
-  s.C = min(ctas, total);  // CTAs with a share: none of them is empty
-  s.q = total / s.C;
-  s.rem = total - s.q * s.C;
-  return s;
-}
 
 struct PagedCursor {
   int r, h, pass;   // request, KV head, pass over its keys
@@ -180,40 +203,70 @@ struct PagedCursor {
   PagedGeom g;
 };
 
-// Shares of this launch, and the cursor at the first tile of share c (c < shares.C, else the cursor is not set).  All
-// lanes of a warp call; lane l looks after requests l, l + 32, ...
-__device__ __forceinline__ PagedShares paged_locate(const PagedArgs& a, int ctas, int cta, PagedCursor& c) {
-  const int lane = threadIdx.x & 31, per = a.H * a.groups;
+// Shares of this launch and the cursor at the first tile of CTA `cta`; false if it has none.  All lanes of a warp call;
+// lane l looks after requests l, l + 32, ...; `warps`: tiles a CTA works on at a time.
+__device__ __forceinline__ bool paged_locate(const PagedArgs& a, int ctas, int cta, int warps, PagedShares& sh, PagedCursor& c) {
+  const int lane = threadIdx.x & 31, per = a.H * a.groups, streams = a.B * per;
   int mine = lane < a.B ? paged_geom(a, lane).tiles : 0;
   int sum = mine;
   for (int r = lane + 32; r < a.B; r += 32) sum += paged_geom(a, r).tiles;
-  const PagedShares sh = paged_shares(__reduce_add_sync(0xffffffffu, sum) * per, ctas);
-  if (cta >= sh.C) return sh;
-  const int x = sh.first(cta);
+  sh.total = __reduce_add_sync(0xffffffffu, sum) * per;
+  sh.C = min(ctas, sh.total);  // CTAs with a share: none of them is empty
+  sh.q = sh.total / sh.C;
+  sh.rem = sh.total - sh.q * sh.C;
+  sh.parts = 0;
+  // aligned: CTAs of a stream of that many tiles, one and its share of those left over (rounded down: all together at
+  // most `ctas`; the factor covers the rounding of the quotient)
+  const float left = (float)(ctas - streams) / (float)sh.total * (1.f - 0x1p-20f);
+  auto ctas_of = [&](int tiles) { return min(1 + (int)((float)tiles * left), (tiles + warps - 1) / warps); };
+  bool aligned = streams <= ctas;
+  if (aligned) {
+    int most = mine > 0 ? (mine + ctas_of(mine) - 1) / ctas_of(mine) : 0;
+    for (int r = lane + 32; r < a.B; r += 32) {
+      const int t = paged_geom(a, r).tiles, n = ctas_of(t);
+      most = max(most, (t + n - 1) / n);
+    }
+    aligned = __reduce_max_sync(0xffffffffu, most) <= sh.q + (sh.q >> 1) + kPagedSlack;
+  }
+  // each request has `per` streams of `unit` places (CTAs or tiles): find the one of place x
+  const int x = aligned ? cta : sh.first(cta);
+  if (!aligned && cta >= sh.C) return false;
   int before = 0;
   for (int base = 0;; base += 32) {
     if (base > 0) mine = base + lane < a.B ? paged_geom(a, base + lane).tiles : 0;
-    int incl = mine * per;
+    const int unit = mine > 0 ? per * (aligned ? ctas_of(mine) : mine) : 0;
+    int incl = unit;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
     const unsigned past = __ballot_sync(0xffffffffu, before + incl > x);
-    if (past != 0u || base + 32 >= a.B) {
-      const int at = past != 0u ? __ffs(past) - 1 : 31;
-      c.r = min(base + at, a.B - 1);
-      before += __shfl_sync(0xffffffffu, incl - mine * per, at);
+    if (past != 0u) {
+      const int at = __ffs(past) - 1;
+      c.r = base + at;
+      before += __shfl_sync(0xffffffffu, incl - unit, at);
       break;
     }
+    if (base + 32 >= a.B) return false;  // aligned: a CTA that no stream needs
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
   c.g = paged_geom(a, c.r);
-  const int sub = (x - before) / c.g.tiles;
-  c.tile = x - before - sub * c.g.tiles;
+  const int unit = aligned ? ctas_of(c.g.tiles) : c.g.tiles;
+  const int sub = (x - before) / unit, i = x - before - sub * unit;
   c.h = sub / a.groups;
   c.pass = sub - c.h * a.groups;
-  return sh;
+  if (aligned) {
+    sh.c0 = cta - i;
+    sh.parts = unit;
+    sh.x = c.tile = c.g.tiles * i / unit;  // fits 31 bits: at most 2^21 tiles and 2^10 CTAs
+    sh.x_end = c.g.tiles * (i + 1) / unit;
+  } else {
+    c.tile = i;
+    sh.x = x;
+    sh.x_end = sh.first(cta + 1);
+  }
+  return true;
 }
 
 __device__ __forceinline__ void paged_next_stream(const PagedArgs& a, PagedCursor& c) {

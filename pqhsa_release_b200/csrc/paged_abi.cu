@@ -81,6 +81,7 @@ static PagedArgs paged_args(const pqhsa_paged_params* p) {
   a.stride_block = p->stride_block; a.stride_head = p->stride_head; a.stride_row = p->stride_row;
   a.B = p->requests; a.H = p->kv_heads; a.G = p->group; a.T = p->query_len; a.R = p->group * p->query_len;
   a.groups = (a.R + kPagedGroupRows - 1) / kPagedGroupRows;
+  a.g_inv = 65536 / p->group + 1;
   a.cap = p->slot_capacity;
   const long long room = p->block_table != nullptr ? (long long)p->max_blocks * p->block_size : p->block_size;
   a.limit = room < a.cap ? (int)room : a.cap;

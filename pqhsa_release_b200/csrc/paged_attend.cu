@@ -49,7 +49,7 @@ __device__ __forceinline__ int merge_at(int entry, int row, int rows, int dim) {
 template <typename E>
 __device__ __forceinline__ void paged_store_row(const PagedArgs& a, int r, int h, int pass, int row, int lane, float M, float L, float4 o) {
   const int full = pass * kPagedGroupRows + row;
-  const int t = full / a.G, hq = h * a.G + full % a.G;
+  const int t = a.token_of(full), hq = h * a.G + full - t * a.G;
   const float inv = L > 0.f || L != L ? 1.f / L : 0.f;  // an empty row is zero, a NaN stays one
   E* dst = static_cast<E*>(a.out) + (int64_t)r * a.o_sr + (int64_t)t * a.o_st + (int64_t)hq * a.o_sh + lane * 4;
   const E v[4] = {from_f<E>(o.x * inv), from_f<E>(o.y * inv), from_f<E>(o.z * inv), from_f<E>(o.w * inv)};
@@ -112,39 +112,43 @@ __device__ __forceinline__ void paged_finish(const PagedArgs& a, const PagedShar
     p.r = c.r;
     p.h = c.h;
     p.pass = c.pass;
-    p.c0 = sh.owner(x - c.tile);
-    p.parts = sh.owner(x - c.tile + c.g.tiles - 1) - p.c0 + 1;
+    p.c0 = sh.parts > 0 ? sh.c0 : sh.owner(x - c.tile);
+    p.parts = sh.parts > 0 ? sh.parts : sh.owner(x - c.tile + c.g.tiles - 1) - p.c0 + 1;
   }
 }
 
-// Folds every `by`-th part of a row of stream p from part `at` on (a warp; eight parts' loads in flight).
-template <int ROWS>
-__device__ __forceinline__ RowSum paged_fold_row(const PagedArgs& a, const PagedPending& p, int row, int at, int by) {
-  constexpr int kAhead = 8;
+// Folds every `by`-th part, from part `at` on, of N rows of stream p (a warp; the loads of kAhead parts in flight).
+template <int ROWS, int N>
+__device__ __forceinline__ void paged_fold_rows(const PagedArgs& a, const PagedPending& p, const int (&row)[N], int at, int by, RowSum (&s)[N]) {
+  constexpr int kAhead = 16 / N;
   const int lane = threadIdx.x & 31;
-  RowSum s;
   for (int p0 = at; p0 < p.parts; p0 += kAhead * by) {
-    float2 x[kAhead];
-    float4 v[kAhead];
+    float2 x[N][kAhead];
+    float4 v[N][kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       const int q = p0 + u * by;
-      x[u] = make_float2(kFloor, 0.f);
-      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (q < p.parts) {
-        const size_t place = (size_t)2 * (p.c0 + q) + (q == 0 ? 1 : 0);
-        x[u] = __ldcg(&a.part_ml[place * kPagedGroupRows + row]);
-        v[u] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + (place * ROWS + row) * kD + lane * 4));
+      const size_t place = (size_t)2 * (p.c0 + q) + (q == 0 ? 1 : 0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        x[i][u] = make_float2(kFloor, 0.f);
+        v[i][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (q < p.parts) {
+          x[i][u] = __ldcg(&a.part_ml[place * kPagedGroupRows + row[i]]);
+          v[i][u] = __ldcg(reinterpret_cast<const float4*>(a.part_acc + (place * ROWS + row[i]) * kD + lane * 4));
+        }
       }
     }
-    float top = x[0].x;
 #pragma unroll
-    for (int u = 1; u < kAhead; ++u) top = fmaxf(top, x[u].x);
-    s.raise(top);
+    for (int i = 0; i < N; ++i) {
+      float top = x[i][0].x;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) s.add(x[u], v[u]);
+      for (int u = 1; u < kAhead; ++u) top = fmaxf(top, x[i][u].x);
+      s[i].raise(top);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) s[i].add(x[i][u], v[i][u]);
+    }
   }
-  return s;
 }
 
 // After the last tile of the CTA (all threads): tickets for its parts, and the fold of the streams it ends.
@@ -163,15 +167,29 @@ __device__ __forceinline__ void paged_fold(const PagedArgs& a, PagedPending* pen
     }
   }
   __syncthreads();
-  // rows of both streams, a warp each, while the parts of a row are few
+  // while the parts of a row are few: the rows of both streams shared out over the warps, one row or two at a time
   constexpr int kFew = 16;
   const auto rows_of = [&](int i) { return pend[i].last != 0 ? min(a.R - pend[i].pass * kPagedGroupRows, kPagedGroupRows) : 0; };
   const int rows0 = pend[0].parts <= kFew ? rows_of(0) : 0, rows1 = pend[1].parts <= kFew ? rows_of(1) : 0;
-  for (int item = warp; item < rows0 + rows1; item += WARPS) {
-    const PagedPending& p = pend[item < rows0 ? 0 : 1];
-    const int row = item < rows0 ? item : item - rows0;
-    const RowSum s = paged_fold_row<ROWS>(a, p, row, 0, 1);
-    paged_store_row<E>(a, p.r, p.h, p.pass, row, lane, s.M, s.L, s.o);
+  if (rows0 + rows1 <= WARPS) {
+    if (warp < rows0 + rows1) {
+      const int i = warp < rows0 ? 0 : 1, row = warp - (i != 0 ? rows0 : 0);
+      const PagedPending& p = pend[i];
+      RowSum s[1];
+      paged_fold_rows<ROWS, 1>(a, p, {row}, 0, 1, s);
+      paged_store_row<E>(a, p.r, p.h, p.pass, row, lane, s[0].M, s[0].L, s[0].o);
+    }
+  } else {
+    const int items0 = (rows0 + 1) / 2, items1 = (rows1 + 1) / 2;
+    for (int item = warp; item < items0 + items1; item += WARPS) {
+      const int i = item < items0 ? 0 : 1, first = (item - (i != 0 ? items0 : 0)) * 2, rows = rows_of(i);
+      const PagedPending& p = pend[i];
+      const int row[2] = {first, min(first + 1, rows - 1)};
+      RowSum s[2];
+      paged_fold_rows<ROWS, 2>(a, p, row, 0, 1, s);
+      paged_store_row<E>(a, p.r, p.h, p.pass, first, lane, s[0].M, s[0].L, s[0].o);
+      if (first + 1 < rows) paged_store_row<E>(a, p.r, p.h, p.pass, first + 1, lane, s[1].M, s[1].L, s[1].o);
+    }
   }
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
@@ -182,8 +200,9 @@ __device__ __forceinline__ void paged_fold(const PagedArgs& a, PagedPending* pen
     const int at = warp % per;
     for (int base = 0; base < rows; base += WARPS / per) {
       const int row = base + warp / per;
-      RowSum s;
-      if (row < rows) s = paged_fold_row<ROWS>(a, p, row, at, per);
+      RowSum one[1];
+      RowSum& s = one[0];
+      if (row < rows) paged_fold_rows<ROWS, 1>(a, p, {row}, at, per, one);
       if (per > 1) {
         __syncthreads();  // the buffer of the round before has been read
         if (lane == 0) ml[warp] = make_float2(s.M, s.L);
@@ -232,10 +251,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const Paged
   if (tid < 2) pend_s[tid].parts = pend_s[tid].last = 0;
   wait_for_grid();
   PagedCursor c;
-  const PagedShares sh = paged_locate(a, gridDim.x, blockIdx.x, c);
-  if (blockIdx.x >= sh.C) return;
-  int x = sh.first(blockIdx.x);
-  const int x_end = sh.first(blockIdx.x + 1);
+  PagedShares sh;
+  if (!paged_locate(a, gridDim.x, blockIdx.x, WARPS, sh, c)) return;
+  int x = sh.x;
+  const int x_end = sh.x_end;
 
   while (true) {
     const int count = min(c.g.tiles - c.tile, x_end - x);  // tiles of this stream in the share
@@ -276,8 +295,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const Paged
       const int row = i / (kD / 4), d = i % (kD / 4) * 4, full = row0 + row;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < rows)
-        v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)c.r * a.q_sr + (int64_t)(full / a.G) * a.q_st +
-                                                  (int64_t)(h * a.G + full % a.G) * a.q_sh + d));
+        v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)c.r * a.q_sr + (int64_t)h * a.G * a.q_sh + a.q_row(full) + d));
       *reinterpret_cast<float4*>(q_s + row * kD + d) = v;
     }
     float slope[OWN], m[OWN], l[OWN], acc[ROWS][4];
@@ -286,8 +304,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const Paged
     for (int i = 0; i < OWN; ++i) {
       const int full = row0 + 4 * i + quarter;
       const bool live = 4 * i + quarter < rows;
-      p_at[i] = live ? c.g.p_first + full / a.G : -1;
-      slope[i] = live && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + full % a.G) : 0.f;
+      p_at[i] = live ? c.g.p_first + a.token_of(full) : -1;
+      slope[i] = live && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + a.head_of(full)) : 0.f;
       m[i] = kFloor;
       l[i] = 0.f;
     }
@@ -416,7 +434,8 @@ static int launch_fp32(const PagedArgs& a, cudaStream_t st) {
                           sizeof(float2) * WARPS * ROWS;
   static_assert(smem <= 225 * 1024, "shared memory of a CTA");
   auto kern = paged_attend_kernel<ROWS, STAGES, WARPS>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  static std::atomic<uint64_t> allowed{0};
+  if (paged_allow_smem((const void*)kern, smem, allowed) != cudaSuccess)
     return check_launch("paged_attend shared memory");
   if (paged_launch(kern, dim3(sm_count()), WARPS * 32, smem, st, 0, a) != cudaSuccess) return check_launch("paged_attend");
   return PQHSA_OK;
@@ -501,10 +520,10 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
   if (tid < 2) pend_s[tid].parts = pend_s[tid].last = 0;
   wait_for_grid();
   PagedCursor c;
-  const PagedShares sh = paged_locate(a, gridDim.x, blockIdx.x, c);
-  if (blockIdx.x >= sh.C) return;
-  int x = sh.first(blockIdx.x);
-  const int x_end = sh.first(blockIdx.x + 1);
+  PagedShares sh;
+  if (!paged_locate(a, gridDim.x, blockIdx.x, kPWarps, sh, c)) return;
+  int x = sh.x;
+  const int x_end = sh.x_end;
 
   // the copies' cursor: tile number `at` of the `at_end` of this warp in stream `ahead`
   PagedCursor ahead = c;
@@ -591,7 +610,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
         const int row = 8 * nb + l4, full = row0 + row;
-        const E* src = base + (int64_t)(full / a.G) * a.q_st + (int64_t)(full % a.G) * a.q_sh + 2 * t4;
+        const E* src = base + a.q_row(full) + 2 * t4;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
           qf[nb][kk][0] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
@@ -603,7 +622,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
         const int row = i >> 4, piece = i & 15, full = row0 + row;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (row < rows)
-          v = __ldg(reinterpret_cast<const uint4*>(base + (int64_t)(full / a.G) * a.q_st + (int64_t)(full % a.G) * a.q_sh) + piece);
+          v = __ldg(reinterpret_cast<const uint4*>(base + a.q_row(full)) + piece);
         *reinterpret_cast<uint4*>(q_s + row * 256 + ((piece ^ (row & 7)) << 4)) = v;
       }
       __syncthreads();
@@ -632,8 +651,8 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
         const int row = 8 * nb + 2 * t4 + j, full = row0 + row;
         m[nb][j] = kFloor;
         l[nb][j] = 0.f;
-        p_at[nb][j] = row < rows ? c.g.p_first + full / a.G : -1;
-        slope[nb][j] = SHAPED && row < rows && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + full % a.G) : 0.f;
+        p_at[nb][j] = row < rows ? c.g.p_first + a.token_of(full) : -1;
+        slope[nb][j] = SHAPED && row < rows && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + a.head_of(full)) : 0.f;
       }
 #pragma unroll
       for (int db = 0; db < 8; ++db)
@@ -853,7 +872,8 @@ static int launch_mma(const PagedArgs& a, cudaStream_t st) {
                           sizeof(float2) * kPWarps * ROWS + (NB > 2 ? ROWS * 256 : 0);
   static_assert(smem <= 225 * 1024 + 512, "shared memory of a CTA");
   auto kern = paged_attend_mma_kernel<E, NB, STAGES, SHAPED>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  static std::atomic<uint64_t> allowed{0};
+  if (paged_allow_smem((const void*)kern, smem, allowed) != cudaSuccess)
     return check_launch("paged_attend shared memory");
   if (paged_launch(kern, dim3(sm_count()), kPThreads, smem, st, 0, a) != cudaSuccess) return check_launch("paged_attend");
   return PQHSA_OK;
@@ -863,14 +883,14 @@ static int launch_mma(const PagedArgs& a, cudaStream_t st) {
 // mass[r, h, i] += sum over the rows of 2^(s - lse): one pass over the scores the attention kernel left (4 bytes per
 // row and key, which come from L2 while the cache rows went past it), the same tiles in equal shares, four keys to a
 // thread.  The rows of a key are added in row order by one thread: no atomics, the same bits every run.
-constexpr int kMassThreads = 128;
+constexpr int kMassThreads = 256;
 __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArgs a) {
   // a.groups is 1 here: one stream per KV head
   PagedCursor c;
-  const PagedShares sh = paged_locate(a, gridDim.x, blockIdx.x, c);
-  if (blockIdx.x >= sh.C) return;
-  int x = sh.first(blockIdx.x);
-  const int x_end = sh.first(blockIdx.x + 1);
+  PagedShares sh;
+  if (!paged_locate(a, gridDim.x, blockIdx.x, kMassThreads / 32, sh, c)) return;
+  int x = sh.x;
+  const int x_end = sh.x_end;
   const int quads = a.tile_log2 - 2;  // log2 of the quads of keys in a tile
   wait_for_grid();  // scores and row sums are there
   while (true) {
@@ -879,7 +899,10 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArg
     for (int i = threadIdx.x; i < count << quads; i += kMassThreads) {
       const int slot = (paged_tile(c.g, c.tile + (i >> quads)) << a.tile_log2) + ((i & ((1 << quads) - 1)) << 2);
       if (slot >= c.g.n) continue;
-      float w[4] = {0.f, 0.f, 0.f, 0.f};
+      float w[4] = {0.f, 0.f, 0.f, 0.f}, old[4];
+      float* to = a.mass + stream * a.cap + slot;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) old[j] = slot + j < c.g.n ? to[j] : 0.f;
       for (int row0 = 0; row0 < a.R; row0 += 4) {
         float4 s[4];
         float z[4];
@@ -897,10 +920,9 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArg
           w[3] += s[j].w == kNegInf ? 0.f : ex2(s[j].w - z[j]);
         }
       }
-      float* to = a.mass + stream * a.cap + slot;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (slot + j < c.g.n && w[j] != 0.f) to[j] += w[j];  // keys no row saw are left as they were
+        if (slot + j < c.g.n && w[j] != 0.f) to[j] = old[j] + w[j];  // keys no row saw are left as they were
     }
     x += count;
     if (x >= x_end) return;
@@ -911,7 +933,7 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArg
 int launch_paged_mass(const PagedArgs& a, cudaStream_t st) {
   PagedArgs b = a;
   b.groups = 1;
-  if (paged_launch(paged_mass_kernel, dim3(sm_count() * 8), kMassThreads, 0, st, 0, b) != cudaSuccess) return check_launch("paged_mass");
+  if (paged_launch(paged_mass_kernel, dim3(sm_count() * 4), kMassThreads, 0, st, 0, b) != cudaSuccess) return check_launch("paged_mass");
   return PQHSA_OK;
 }
 

@@ -413,7 +413,8 @@ int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaS
   const bool resident = share <= kEvShare;
   const size_t smem = resident ? sizeof(uint32_t) * (size_t)share : 0;
   auto kern = resident ? evict_select_kernel<true> : evict_select_kernel<false>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  static std::atomic<uint64_t> allowed{0};
+  if (resident && paged_allow_smem((const void*)kern, sizeof(uint32_t) * kEvShare, allowed) != cudaSuccess)
     return check_launch("evict_select shared memory");
   if (paged_launch(kern, dim3(ranks, a.B * a.H), kEvThreads, smem, st, ranks, a, e) != cudaSuccess) return check_launch("evict_select");
   const int most = e.budget < a.limit ? (e.budget < a.limit - e.budget ? e.budget : a.limit - e.budget) : 0;

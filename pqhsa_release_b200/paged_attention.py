@@ -18,7 +18,8 @@ from . import _lib
 from .device_index import _DTYPE_CODE
 
 MAX_QUERY_LEN, MAX_GROUP, MAX_ROWS = 8, 16, 64
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_is_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 class PagedAttention:
@@ -66,25 +67,28 @@ class PagedAttention:
             if tuple(alibi_slopes.shape) != (self.Hq,):
                 raise ValueError(f"alibi_slopes must have one entry per query head, got {tuple(alibi_slopes.shape)}")
             self.alibi_slopes = alibi_slopes.detach().to(device=self.device, dtype=torch.float32).contiguous().clone()
-        p = self.p = _lib.PagedParams()
-        p.abi_version, p.dtype, p.head_dim = _lib.ABI_VERSION, _DTYPE_CODE[dtype], _lib.HEAD_DIM
-        p.requests, p.kv_heads, p.group, p.query_len = self.max_requests, self.H, self.G, self.max_query_len
-        p.slot_capacity = self.token_capacity
-        p.scale, p.softcap, p.window, p.sink_tokens = scale, float(softcap), int(window), int(sink_tokens)
-        p.alibi_slopes = self.alibi_slopes.data_ptr() if self.alibi_slopes is not None else None
-        self._ref = C.byref(p)
+        # one argument block per operator (each keeps the sizes of its last call), the cache's part the same in all
+        self.p, self._append_p, self._evict_p = _lib.PagedParams(), _lib.PagedParams(), _lib.PagedParams()
+        for p in (self.p, self._append_p, self._evict_p):
+            p.abi_version, p.dtype, p.head_dim = _lib.ABI_VERSION, _DTYPE_CODE[dtype], _lib.HEAD_DIM
+            p.requests, p.kv_heads, p.group, p.query_len = self.max_requests, self.H, self.G, self.max_query_len
+            p.slot_capacity = self.token_capacity
+            p.scale, p.softcap, p.window, p.sink_tokens = scale, float(softcap), int(window), int(sink_tokens)
+        self.p.alibi_slopes = self.alibi_slopes.data_ptr() if self.alibi_slopes is not None else None
+        self._ref, self._append_ref, self._evict_ref = C.byref(self.p), C.byref(self._append_p), C.byref(self._evict_p)
         self._bytes = []
         for mass in (None, 1):
-            p.mass = mass
+            self.p.mass = mass
             n = int(_lib.lib.pqhsa_paged_workspace_bytes(self._ref))
             if n == 0:
                 raise ValueError(_lib.lib.pqhsa_last_error_string().decode("utf-8", "replace"))
             self._bytes.append(n)
-        p.mass = None
+        self.p.mass = None
         self._ws: dict = {}
         self._kept: list = []
         self._kv_keepalive = None
         self._rows = 0  # requests the bound cache addresses
+        self._forward_shape = self._append_shape = None  # shapes the blocks are set for (contiguous rows), or None
 
     # ---- cache ----------------------------------------------------------------------------------------
     def bind_kv_paged(self, kv_cache: torch.Tensor, block_table: torch.Tensor) -> None:
@@ -95,7 +99,7 @@ class PagedAttention:
         self._check(block_table, "block_table", torch.int32)
         if block_table.dim() != 2 or not block_table.is_contiguous() or block_table.numel() == 0:
             raise ValueError("block_table must be a contiguous int32 [requests, max_blocks] tensor")
-        p, D = self.p, _lib.HEAD_DIM
+        D = _lib.HEAD_DIM
         if kv_cache.dim() == 5:
             if kv_cache.shape[0] != 2 or kv_cache.shape[4] != D or kv_cache.shape[3] != self.H or kv_cache.stride(4) != 1:
                 raise ValueError(f"5-D KV pages must be [2, blocks, block_size, {self.H}, 128] with contiguous rows")
@@ -108,8 +112,7 @@ class PagedAttention:
             strides = kv_cache.stride(0), kv_cache.stride(1), kv_cache.stride(2)
         else:
             raise ValueError(f"unsupported FLASH_ATTN kv_cache shape {tuple(kv_cache.shape)}")
-        self._bind(base, base + off, nb, bs, strides)
-        p.block_table, p.max_blocks = block_table.data_ptr(), block_table.shape[1]
+        self._bind(base, base + off, nb, bs, strides, block_table.data_ptr(), block_table.shape[1])
         self._rows = block_table.shape[0]
         self._kv_keepalive = (kv_cache, block_table)
 
@@ -121,20 +124,22 @@ class PagedAttention:
             raise ValueError(f"keys and values must be [B, {self.H}, capacity, 128]")
         if keys.shape != values.shape or keys.stride() != values.stride() or keys.stride(-1) != 1:
             raise ValueError("keys and values must have the same shape and strides with contiguous rows")
-        self._bind(keys.data_ptr(), values.data_ptr(), keys.shape[0], keys.shape[2], (keys.stride(0), keys.stride(1), keys.stride(2)))
-        self.p.block_table, self.p.max_blocks = None, 0
+        self._bind(keys.data_ptr(), values.data_ptr(), keys.shape[0], keys.shape[2],
+                   (keys.stride(0), keys.stride(1), keys.stride(2)), None, 0)
         self._rows = keys.shape[0]
         self._kv_keepalive = (keys, values)
 
-    def _bind(self, k: int, v: int, blocks: int, block_size: int, strides) -> None:
+    def _bind(self, k: int, v: int, blocks: int, block_size: int, strides, table, max_blocks: int) -> None:
         if blocks < 1 or block_size < 1:
             raise ValueError("the KV cache is empty")
         a = 4 if self.dtype == torch.float32 else 8
         if (k | v) & 15 or any(s % a for s in strides):
             raise ValueError("KV rows must be 16-byte aligned")
-        p = self.p
-        p.k_base, p.v_base, p.num_blocks, p.block_size = k, v, blocks, block_size
-        p.stride_block, p.stride_head, p.stride_row = strides
+        for p in (self.p, self._append_p, self._evict_p):
+            p.k_base, p.v_base, p.num_blocks, p.block_size = k, v, blocks, block_size
+            p.stride_block, p.stride_head, p.stride_row = strides
+            p.block_table, p.max_blocks = table, max_blocks
+        self._forward_shape = self._append_shape = None
 
     # ---- checks and scratch ------------------------------------------------------------------------------
     def _check(self, t: torch.Tensor, name: str, dtype: torch.dtype) -> None:
@@ -142,47 +147,52 @@ class PagedAttention:
             raise ValueError(f"{name} must be a {dtype} tensor on {self.device}, got {t.dtype} on {t.device}")
 
     def _per_request(self, t: torch.Tensor, name: str, B: int) -> int:
-        if t.dtype is not torch.int32 or t.device != self.device or t.dim() != 1 or t.shape[0] != B or not t.is_contiguous():
+        if t.dtype is not torch.int32 or t.get_device() != self._index or t.shape != (B,) or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous int32 tensor of {B} entries on {self.device}")
         return t.data_ptr()
 
     def _per_slot(self, t: torch.Tensor, name: str, dtype: torch.dtype, B: int) -> int:
-        if (t.dtype is not dtype or t.device != self.device or t.dim() != 3 or t.shape[0] < B or t.shape[1] != self.H
-                or t.shape[2] != self.token_capacity or not t.is_contiguous()):
+        shape = t.shape
+        if (t.dtype is not dtype or t.get_device() != self._index or len(shape) != 3 or shape[0] < B
+                or shape[1:] != (self.H, self.token_capacity) or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous {dtype} [>= {B}, {self.H}, {self.token_capacity}] tensor on {self.device}")
         return t.data_ptr()
 
-    def _rows_of(self, t: torch.Tensor, name: str, heads: int):
-        """(address, strides of request, token, head, B, T) of ``[B, heads, 128]`` or ``[B, T, heads, 128]`` rows."""
-        if t.dtype is not self.dtype or t.device != self.device:
-            raise ValueError(f"{name} must be a {self.dtype} tensor on {self.device}, got {t.dtype} on {t.device}")
-        shape, st = t.shape, t.stride()
-        if len(shape) == 3:
-            B, T, s = shape[0], 1, (st[0], 0, st[1])
-        elif len(shape) == 4:
-            B, T, s = shape[0], shape[1], (st[0], st[1], st[2])
-        else:
+    def _tokens(self, shape, name: str, heads: int) -> tuple[int, int]:
+        """(requests, tokens) of a ``[B, heads, 128]`` or ``[B, T, heads, 128]`` shape this layer can serve."""
+        if len(shape) not in (3, 4):
             raise ValueError(f"{name} must be [requests, heads, 128] or [requests, tokens, heads, 128]")
-        if shape[-2] != heads or shape[-1] != _lib.HEAD_DIM or st[-1] != 1:
-            raise ValueError(f"{name} must have {heads} heads of contiguous 128-element rows, got {tuple(shape)}")
+        B, T = shape[0], shape[1] if len(shape) == 4 else 1
+        if shape[-2] != heads or shape[-1] != _lib.HEAD_DIM:
+            raise ValueError(f"{name} must have {heads} heads of 128 elements, got {tuple(shape)}")
         if B > self.max_requests or B > self._rows:
             raise ValueError(f"{B} requests: the layer was made for {self.max_requests}, the bound cache addresses {self._rows}")
         if not 1 <= T <= self.max_query_len:
             raise ValueError(f"{T} query tokens per request: the layer was made for 1..{self.max_query_len}")
-        a, low = t.data_ptr(), 3 if self.dtype is torch.float32 else 7
-        if (s[0] | s[1] | s[2]) & low:
-            s = (s[0] if B > 1 else 0, s[1] if T > 1 else 0, s[2] if heads > 1 else 0)  # a single row has no stride
-        if a & 15 or ((s[0] | s[1] | s[2]) & low):
+        return B, T
+
+    def _rows_at(self, t: torch.Tensor, name: str) -> int:
+        if t.dtype is not self.dtype or t.get_device() != self._index:
+            raise ValueError(f"{name} must be a {self.dtype} tensor on {self.device}, got {t.dtype} on {t.device}")
+        a = t.data_ptr()
+        if a & 15:
             raise ValueError(f"rows of {name} must be 16-byte aligned")
-        return a, s, B, T
+        return a
+
+    def _strides_of(self, t: torch.Tensor, name: str) -> tuple[int, int, int]:
+        """Element strides from one request, token and head to the next."""
+        shape, st = t.shape, t.stride()
+        s = (st[0], 0, st[1]) if len(shape) == 3 else (st[0], st[1], st[2])
+        s = tuple(x if n > 1 else 0 for x, n in zip(s, (shape[0], shape[1] if len(shape) == 4 else 1, shape[-2])))  # one row has no stride
+        if st[-1] != 1 or (s[0] | s[1] | s[2]) & (3 if self.dtype is torch.float32 else 7):
+            raise ValueError(f"rows of {name} must be contiguous and 16-byte aligned")
+        return s
 
     def _scratch(self, kind: str, nbytes: int) -> tuple[int, int]:
         """(address, stream) of this stream's (or this capture's) scratch memory of that kind."""
         stream = _raw_stream(self._index)
-        key = (kind, stream)
-        capturing = torch.cuda.is_current_stream_capturing()
-        if capturing:
-            key = (kind, stream, _lib.lib.pqhsa_stream_capture_id(stream))
+        capturing = _is_capturing()
+        key = (kind, stream, _lib.lib.pqhsa_stream_capture_id(stream)) if capturing else (kind, stream)
         t = self._ws.get(key)
         if t is None or t.numel() < nbytes:
             if capturing and t is not None:
@@ -192,15 +202,16 @@ class PagedAttention:
                 t[:4096].zero_()  # the kernels' counters
         return t.data_ptr(), stream
 
-    def _bound(self) -> None:
-        if self._kv_keepalive is None:
-            raise RuntimeError("bind_kv_paged or bind_kv_contiguous must be called first")
-
-    def _positions(self, B: int, key_pos, query_pos, mass) -> None:
-        p = self.p
+    def _positions(self, p, B: int, key_pos, query_pos, mass) -> None:
         p.key_pos = None if key_pos is None else self._per_slot(key_pos, "key_pos", torch.int32, B)
         p.query_pos = None if query_pos is None else self._per_request(query_pos, "query_pos", B)
         p.mass = None if mass is None else self._per_slot(mass, "mass", torch.float32, B)
+
+    def _call(self, name: str, *args) -> None:
+        """A library call with this layer's device current; the last argument of every entry point is the stream."""
+        rc = getattr(_lib.lib, name)(*args)
+        if rc != 0:
+            raise _lib.PqhsaError(name, rc, _lib.lib.pqhsa_last_error_string().decode("utf-8", "replace"))
 
     # ---- calls ---------------------------------------------------------------------------------------------
     def forward(self, q: torch.Tensor, seq_lens: torch.Tensor, *, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
@@ -214,40 +225,39 @@ class PagedAttention:
         position of the request's current document.  ``key_pos`` int32 ``[>= B, Hkv, token_capacity]`` with ``query_pos``
         int32 ``[B]`` (position of the last query token): the slots' positions, after an eviction.  ``mass`` float32, same shape as
         key_pos: every slot's attention weights of this call are added to it."""
-        self._bound()
-        p, Hq = self.p, self.Hq
-        p.q, s, B, T = self._rows_of(q, "q", Hq)
-        p.q_stride_request, p.q_stride_token, p.q_stride_head = s
-        if key_pos is not None and query_pos is None:
-            raise ValueError("key_pos needs query_pos")
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.forward(q, seq_lens, out=out, lse=lse, first_key=first_key, key_pos=key_pos, query_pos=query_pos, mass=mass)
+        if self._kv_keepalive is None:
+            raise RuntimeError("bind_kv_paged or bind_kv_contiguous must be called first")
+        p, shape = self.p, q.shape
         if out is None:
-            out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-        elif out.shape != q.shape:
+            out = torch.empty(shape, dtype=self.dtype, device=self.device)
+        elif out.shape != shape:
             raise ValueError("out must match q in shape")
-        p.out, (p.out_stride_request, p.out_stride_token, p.out_stride_head), _, _ = self._rows_of(out, "out", Hq)
+        p.q, p.out = self._rows_at(q, "q"), self._rows_at(out, "out")
+        even = q.is_contiguous() and out.is_contiguous()
+        if not even or shape != self._forward_shape:
+            p.requests, p.query_len = self._tokens(shape, "q", self.Hq)
+            p.q_stride_request, p.q_stride_token, p.q_stride_head = self._strides_of(q, "q")
+            p.out_stride_request, p.out_stride_token, p.out_stride_head = self._strides_of(out, "out")
+            self._forward_shape = shape if even else None
+        B = shape[0]
+        p.seq_lens = self._per_request(seq_lens, "seq_lens", B)
         if lse is None:
             p.lse = None
         else:
-            if lse.dtype is not torch.float32 or lse.device != self.device or lse.shape != q.shape[:-1] or not lse.is_contiguous():
-                raise ValueError(f"lse must be a contiguous float32 tensor of shape {tuple(q.shape[:-1])} on {self.device}")
+            if lse.dtype is not torch.float32 or lse.get_device() != self._index or lse.shape != shape[:-1] or not lse.is_contiguous():
+                raise ValueError(f"lse must be a contiguous float32 tensor of shape {tuple(shape[:-1])} on {self.device}")
             p.lse = lse.data_ptr()
-        p.requests, p.query_len = B, T
-        p.seq_lens = self._per_request(seq_lens, "seq_lens", B)
         p.first_key = None if first_key is None else self._per_request(first_key, "first_key", B)
-        self._positions(B, key_pos, query_pos, mass)
-        self._launch_attention()
-        return out
-
-    def _launch_attention(self) -> None:
-        if torch._C._cuda_getDevice() != self._index:
-            with torch.cuda.device(self._index):
-                return self._launch_attention()
-        p = self.p
-        p.workspace_bytes = n = self._bytes[0 if p.mass is None else 1]
+        if key_pos is not None and query_pos is None:
+            raise ValueError("key_pos needs query_pos")
+        self._positions(p, B, key_pos, query_pos, mass)
+        p.workspace_bytes = n = self._bytes[0 if mass is None else 1]
         p.workspace, stream = self._scratch("attention", n)
-        rc = _lib.lib.pqhsa_paged_attention(self._ref, stream)
-        if rc != 0:
-            raise _lib.PqhsaError("pqhsa_paged_attention", rc, _lib.lib.pqhsa_last_error_string().decode("utf-8", "replace"))
+        self._call("pqhsa_paged_attention", self._ref, stream)
+        return out
 
     def append(self, keys: torch.Tensor, values: torch.Tensor, seq_lens: torch.Tensor, *, new_lens: torch.Tensor | None = None,
                key_pos: torch.Tensor | None = None, query_pos: torch.Tensor | None = None,
@@ -256,21 +266,29 @@ class PagedAttention:
         their positions (``query_pos`` is that of the last; without it, the slots) in ``key_pos`` and no weight yet in
         ``mass``.  Returns ``new_lens`` = lengths + T, ``seq_lens`` itself if not given.  A negative length is an idle
         request; rows that do not fit are dropped."""
-        self._bound()
-        p = self.p
-        k, s, B, T = self._rows_of(keys, "keys", self.H)
-        if values.shape != keys.shape or values.stride() != keys.stride():
-            raise ValueError("keys and values must have the same shape and strides")
-        v, _, _, _ = self._rows_of(values, "values", self.H)
-        p.q_stride_request, p.q_stride_token, p.q_stride_head = s
-        p.requests, p.query_len = B, T
-        p.seq_lens = self._per_request(seq_lens, "seq_lens", B)
-        new_lens = seq_lens if new_lens is None else new_lens
-        to = self._per_request(new_lens, "new_lens", B)
-        self._positions(B, key_pos, query_pos, mass)
-        with torch.cuda.device(self._index):
-            _lib.call("pqhsa_paged_append", self._ref, k, v, to, _raw_stream(self._index))
-        return new_lens
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.append(keys, values, seq_lens, new_lens=new_lens, key_pos=key_pos, query_pos=query_pos, mass=mass)
+        if self._kv_keepalive is None:
+            raise RuntimeError("bind_kv_paged or bind_kv_contiguous must be called first")
+        p, shape = self._append_p, keys.shape
+        k, v = self._rows_at(keys, "keys"), self._rows_at(values, "values")
+        if values.shape != shape:
+            raise ValueError("keys and values must have the same shape")
+        even = keys.is_contiguous() and values.is_contiguous()
+        if not even or shape != self._append_shape:
+            p.requests, p.query_len = self._tokens(shape, "keys", self.H)
+            s = self._strides_of(keys, "keys")
+            if self._strides_of(values, "values") != s:
+                raise ValueError("keys and values must have the same strides")
+            p.q_stride_request, p.q_stride_token, p.q_stride_head = s
+            self._append_shape = shape if even else None
+        B = shape[0]
+        p.seq_lens = at = self._per_request(seq_lens, "seq_lens", B)
+        to = at if new_lens is None else self._per_request(new_lens, "new_lens", B)
+        self._positions(p, B, key_pos, query_pos, mass)
+        self._call("pqhsa_paged_append", self._append_ref, k, v, to, _raw_stream(self._index))
+        return seq_lens if new_lens is None else new_lens
 
     def evict(self, seq_lens: torch.Tensor, *, mass: torch.Tensor, key_pos: torch.Tensor, query_pos: torch.Tensor, budget: int,
               recent: int = 0, new_lens: torch.Tensor | None = None, new_mass: torch.Tensor | None = None,
@@ -281,32 +299,32 @@ class PagedAttention:
         too unless ``new_mass`` / ``new_pos`` are given).  Returns ``new_lens``, ``seq_lens`` itself if not given.
         ``source`` int32 ``[B, Hkv, budget]`` receives the former slot of every kept slot (-1 past the end).  The pages
         of a request must be its own; whole pages behind the new length may be freed."""
-        self._bound()
-        p = self.p
-        budget, recent = int(budget), int(recent)
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.evict(seq_lens, mass=mass, key_pos=key_pos, query_pos=query_pos, budget=budget, recent=recent,
+                                  new_lens=new_lens, new_mass=new_mass, new_pos=new_pos, source=source)
+        if self._kv_keepalive is None:
+            raise RuntimeError("bind_kv_paged or bind_kv_contiguous must be called first")
+        p = self._evict_p
         if not 1 <= budget <= 1 << 24 or recent < 0 or p.sink_tokens + recent > budget:
             raise ValueError(f"need budget >= 1 and sink_tokens + recent <= budget, got {budget}, {p.sink_tokens} + {recent}")
         B = seq_lens.shape[0]
         if B > self.max_requests or B > self._rows:
             raise ValueError(f"{B} requests: the layer was made for {self.max_requests}, the bound cache addresses {self._rows}")
-        if B == 0:
-            return seq_lens if new_lens is None else new_lens
         p.requests, p.query_len = B, 1
-        p.seq_lens = self._per_request(seq_lens, "seq_lens", B)
-        new_lens = seq_lens if new_lens is None else new_lens
-        to = self._per_request(new_lens, "new_lens", B)
-        self._positions(B, key_pos, query_pos, mass)
+        p.seq_lens = at = self._per_request(seq_lens, "seq_lens", B)
+        to = at if new_lens is None else self._per_request(new_lens, "new_lens", B)
+        self._positions(p, B, key_pos, query_pos, mass)
         nm = p.mass if new_mass is None else self._per_slot(new_mass, "new_mass", torch.float32, B)
         npos = p.key_pos if new_pos is None else self._per_slot(new_pos, "new_pos", torch.int32, B)
-        with torch.cuda.device(self._index):
-            n = 4 * B * self.H * (2 * budget + 8)
-            scratch, stream = self._scratch("evict", n + 4 * B * self.H * budget)
-            if source is None:
-                src = scratch + n
-            else:
-                if (source.dtype is not torch.int32 or source.device != self.device or tuple(source.shape) != (B, self.H, budget)
-                        or not source.is_contiguous()):
-                    raise ValueError(f"source must be a contiguous int32 [{B}, {self.H}, {budget}] tensor on {self.device}")
-                src = source.data_ptr()
-            _lib.call("pqhsa_paged_evict", self._ref, budget, recent, to, nm, npos, src, scratch, stream)
-        return new_lens
+        n = 4 * B * self.H * (2 * budget + 8)
+        scratch, stream = self._scratch("evict", n + 4 * B * self.H * budget)
+        if source is None:
+            src = scratch + n
+        else:
+            if (source.dtype is not torch.int32 or source.get_device() != self._index or source.shape != (B, self.H, budget)
+                    or not source.is_contiguous()):
+                raise ValueError(f"source must be a contiguous int32 [{B}, {self.H}, {budget}] tensor on {self.device}")
+            src = source.data_ptr()
+        self._call("pqhsa_paged_evict", self._evict_ref, int(budget), int(recent), to, nm, npos, src, scratch, stream)
+        return seq_lens if new_lens is None else new_lens
