@@ -1,0 +1,132 @@
+"""Decode attention over a cache that stays within a budget by dropping the keys that have gathered the least attention
+weight: the other way, next to the IVF-PQ index, of bounding what a long context costs per step.  Exact attention over
+the keys that are left, no approximation of the others.
+
+Same call forms as :class:`~pqhsa_release_b200.decode_adapter.IVFPQDecodeAttentionAdapter`:
+
+    keys / values : [batch, kv_heads, seq, 128]         queries : [batch, query_heads, 128]
+
+``ValueError`` for shapes, ``RuntimeError`` for use before ``build_cache``.  The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .decode_adapter import DecodeAttentionOutput, _squeeze_decode_token
+from .paged_attention import MAX_QUERY_LEN, MAX_ROWS, PagedAttention
+
+
+class EvictingCacheAdapter:
+    """Up to ``budget + interval`` keys per (request, KV head); once that many are there, an eviction keeps ``budget``:
+    the first ``sink_tokens`` and last ``recent`` positions and those of the largest accumulated weight.  ``softcap``,
+    ``alibi_slopes`` and ``window`` as for :class:`PagedAttention`."""
+
+    def __init__(self, *, num_query_heads: int, num_kv_heads: int, budget: int, interval: int = 256, sink_tokens: int = 4,
+                 recent: int = 128, scale: float | None = None, softcap: float = 0.0,
+                 alibi_slopes: torch.Tensor | None = None, window: int = 0) -> None:
+        if num_kv_heads < 1 or num_query_heads % num_kv_heads != 0:
+            raise ValueError("GQA requires num_query_heads % num_kv_heads == 0")
+        if budget < 1 or interval < 1 or sink_tokens < 0 or recent < 0 or sink_tokens + recent > budget:
+            raise ValueError("need budget >= 1, interval >= 1 and sink_tokens + recent <= budget")
+        self.num_query_heads, self.num_kv_heads = int(num_query_heads), int(num_kv_heads)
+        self.budget, self.interval, self.recent = int(budget), int(interval), int(recent)
+        self._kw = dict(scale=scale, softcap=softcap, alibi_slopes=alibi_slopes, window=window, sink_tokens=int(sink_tokens))
+        self.attention: PagedAttention | None = None
+        self.length = 0      # keys held per (request, KV head)
+        self.position = 0    # tokens seen
+        self.evictions = 0
+
+    # ---- cache -------------------------------------------------------------------------------------------
+    def _layer(self, keys: torch.Tensor, values: torch.Tensor) -> None:
+        """Bind a layer to these contiguous buffers; positions and weights are [batch, kv_heads, capacity] as they."""
+        B, H, cap, _ = keys.shape
+        group = self.num_query_heads // H
+        self.attention = PagedAttention(num_query_heads=self.num_query_heads, num_kv_heads=H, max_requests=B, token_capacity=cap,
+                                        dtype=keys.dtype, device=keys.device, max_query_len=min(MAX_QUERY_LEN, MAX_ROWS // group), **self._kw)
+        self.attention.bind_kv_contiguous(keys, values)
+        self.keys, self.values = keys, values
+
+    def build_cache(self, keys: torch.Tensor, values: torch.Tensor, queries: torch.Tensor | None = None) -> "EvictingCacheAdapter":
+        """The prompt's keys and values (copied).  ``queries`` ``[batch, query_heads, W, 128]``: those of its last W
+        tokens, whose attention weights choose what a prompt longer than the budget keeps; without them only the last
+        and the first positions are told apart from the rest, of which the lowest stay."""
+        if keys.ndim != 4 or values.ndim != 4 or keys.shape != values.shape or keys.shape[1] != self.num_kv_heads or keys.shape[3] != _lib.HEAD_DIM:
+            raise ValueError(f"keys and values must be [batch, {self.num_kv_heads}, seq, 128]")
+        B, H, S, D = keys.shape
+        if S < 1:
+            raise ValueError("the prompt is empty")
+        if queries is not None and (queries.ndim != 4 or queries.shape[:2] != (B, self.num_query_heads) or queries.shape[3] != D
+                                    or not 1 <= queries.shape[2] <= S or queries.dtype != keys.dtype):
+            raise ValueError(f"queries must be [{B}, {self.num_query_heads}, 1..{S}, 128] in the keys' dtype")
+        dev, room = keys.device, self.budget + self.interval
+
+        def buffers(cap):
+            k, v = (torch.zeros(B, H, cap, D, dtype=keys.dtype, device=dev) for _ in range(2))
+            return k, v, torch.zeros(B, H, cap, dtype=torch.int32, device=dev), torch.zeros(B, H, cap, device=dev)
+
+        k, v, self.positions, self.weights = buffers(max(S, room))
+        k[:, :, :S], v[:, :, :S] = keys, values
+        self.positions[:] = torch.arange(k.shape[2], dtype=torch.int32, device=dev)
+        self._layer(k, v)
+        self.lens = torch.full((B,), S, dtype=torch.int32, device=dev)
+        self.query_pos = torch.full((B,), S - 1, dtype=torch.int32, device=dev)
+        self.length = self.position = S
+        if queries is not None:
+            W, step = queries.shape[2], self.attention.max_query_len
+            for lo in range(0, W, step):  # a few tokens at a time, each seeing what lies before it
+                hi = min(lo + step, W)
+                at = torch.full_like(self.query_pos, S - W + hi - 1)
+                self.attention.forward(queries[:, :, lo:hi].transpose(1, 2), self.lens, key_pos=self.positions, query_pos=at,
+                                       mass=self.weights)
+        if S >= room:
+            self._evict()
+            if S > room:  # the long buffers are not needed any more
+                small = buffers(room)
+                for big, to in zip((self.keys, self.values, self.positions, self.weights), small):
+                    to[:, :, : self.length] = big[:, :, : self.length]
+                self.positions, self.weights = small[2], small[3]
+                self._layer(small[0], small[1])
+        return self
+
+    def _evict(self) -> None:
+        self.attention.evict(self.lens, mass=self.weights, key_pos=self.positions, query_pos=self.query_pos, budget=self.budget,
+                             recent=self.recent)
+        self.length = min(self.length, self.budget)
+        self.evictions += 1
+
+    def _ready(self) -> PagedAttention:
+        if self.attention is None:
+            raise RuntimeError("build_cache must be called before the cache is used")
+        return self.attention
+
+    # ---- decode -------------------------------------------------------------------------------------------
+    def append(self, keys: torch.Tensor, values: torch.Tensor) -> None:
+        """One token per request, ``[batch, kv_heads, 128]`` (or with a token dimension of one)."""
+        att = self._ready()
+        keys, values = _squeeze_decode_token(keys, "keys"), _squeeze_decode_token(values, "values")
+        if keys.shape != (self.keys.shape[0], self.num_kv_heads, _lib.HEAD_DIM) or values.shape != keys.shape:
+            raise ValueError(f"keys and values must be [{self.keys.shape[0]}, {self.num_kv_heads}, 128]")
+        if self.length >= self.budget + self.interval:
+            self._evict()
+        self.query_pos.add_(1)
+        att.append(keys.contiguous(), values.contiguous(), self.lens, key_pos=self.positions, query_pos=self.query_pos, mass=self.weights)
+        self.length += 1
+        self.position += 1
+
+    def forward(self, queries: torch.Tensor) -> DecodeAttentionOutput:
+        """The last token's attention; its weights are accumulated."""
+        att = self._ready()
+        if queries.ndim != 3 or queries.shape != (self.keys.shape[0], self.num_query_heads, _lib.HEAD_DIM):
+            raise ValueError(f"queries must be [{self.keys.shape[0]}, {self.num_query_heads}, 128]")
+        return DecodeAttentionOutput(context=att.forward(queries, self.lens, key_pos=self.positions, query_pos=self.query_pos,
+                                                         mass=self.weights))
+
+    def decode_step(self, queries: torch.Tensor, keys: torch.Tensor | None = None, values: torch.Tensor | None = None, *,
+                    append_kv: bool = True) -> DecodeAttentionOutput:
+        if append_kv:
+            if keys is None or values is None:
+                raise ValueError("keys and values are required when append_kv=True")
+            self.append(keys, values)
+        return self.forward(queries)

@@ -5,7 +5,8 @@ batch driver ``pq_hsa_batch_decode.py`` (:383-432), on the B200 library.
 
 The wrapped ``FlashAttentionImpl.forward`` keeps vLLM's signature and writes its result in place
 into ``output``.  A step is taken by the PQ path only if it is a pure single-token decode step of
-requests that are long enough; everything else goes to the original forward.  Errors re-raise
+requests that are long enough; everything else goes to the original forward, or with ``PQ_HSA_DENSE=1``, if it is a
+decode step, to this library's dense attention over the same pages.  Errors re-raise
 unless ``PQ_HSA_FALLBACK=1`` (then the original forward runs instead).
 
 Where the reference keeps one sidecar per (layer, request) and loops the requests in Python, a
@@ -27,6 +28,7 @@ STATS: dict[str, int] = {"pq_steps": 0, "dense_steps": 0, "builds": 0, "flushes"
                          "restores": 0, "evictions": 0, "kv_writes": 0}
 _REJECTS: dict[str, int] = {}
 _LAYERS: dict[int, Any] = {}  # id(layer) -> PagedBatchEngine
+_DENSE: dict[tuple, Any] = {}  # (id(layer), requests, query tokens, slots, dtype) -> PagedAttention, kept for captured graphs
 
 
 def reject(reason: str) -> bool:
@@ -41,6 +43,7 @@ def rejects() -> dict[str, int]:
 def reset() -> None:
     """Forget every layer's engine (tests; a worker that reloads its model)."""
     _LAYERS.clear()
+    _DENSE.clear()
     _REJECTS.clear()
     for k in STATS:
         STATS[k] = 0
@@ -324,8 +327,78 @@ def run_pq_decode_mq(impl, layer, query, key, value, kv_cache, attn_metadata, ou
     return output
 
 
+def dense_enabled() -> bool:
+    """PQ_HSA_DENSE=1 (default 0): decode steps that the PQ path does not take - contexts too short for an index, a batch
+    with such a request, requests without ids - run on this library's dense kernel instead of the original forward."""
+    return os.environ.get("PQ_HSA_DENSE", "0") == "1"
+
+
+def should_dense_decode(impl, kv_cache, attn_metadata) -> bool:
+    """A pure decode step (the same few query tokens for every request) over 128-dimensional heads in a 16- or 32-bit
+    cache; anything else stays with the original forward."""
+    import torch
+
+    from ..paged_attention import MAX_GROUP, MAX_QUERY_LEN, MAX_ROWS
+    from ..paged_kv import kv_cache_dims
+
+    if attn_metadata is None or getattr(attn_metadata, "use_cascade", False) or getattr(attn_metadata, "seq_lens", None) is None:
+        return reject("dense_metadata")
+    T, n = int(getattr(attn_metadata, "max_query_len", 0)), int(attn_metadata.seq_lens.shape[0])
+    if not 1 <= T <= MAX_QUERY_LEN or n < 1 or int(getattr(attn_metadata, "num_actual_tokens", 0)) != n * T:
+        return reject("dense_query_len")
+    if getattr(impl, "attn_type", "decoder") not in ("decoder",) or not isinstance(kv_cache, torch.Tensor) or kv_cache.dim() not in (4, 5):
+        return reject("dense_layer")
+    _, heads, dim = kv_cache_dims(kv_cache)
+    group = impl.num_heads // max(impl.num_kv_heads, 1)
+    if dim != 128 or heads != impl.num_kv_heads or impl.num_heads != group * impl.num_kv_heads or group > MAX_GROUP or group * T > MAX_ROWS:
+        return reject("dense_heads")
+    if kv_cache.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        return reject("dense_dtype")
+    left, right = tuple(getattr(impl, "sliding_window", None) or (-1, -1))
+    if right > 0 or getattr(impl, "sinks", None) is not None:
+        return reject("dense_scores")
+    return True
+
+
+def run_dense_decode(impl, layer, query, key, value, kv_cache, attn_metadata, output):
+    """The step's exact attention over the pages, with the layer's own window, cap and distance bias, into ``output``."""
+    import torch
+
+    from ..paged_attention import PagedAttention
+    from ..paged_kv import kv_cache_dims
+
+    T, n = int(attn_metadata.max_query_len), int(attn_metadata.seq_lens.shape[0])
+    write_step_kv(key, value, kv_cache, attn_metadata)
+    table = attn_metadata.block_table[:n]
+    if table.dtype != torch.int32 or not table.is_contiguous():
+        table = table.to(torch.int32).contiguous()
+    slots = int(table.shape[1]) * kv_cache_dims(kv_cache)[0]
+    size = (id(layer), 1 << (n - 1).bit_length(), T, slots, kv_cache.dtype)
+    att = _DENSE.get(size)
+    if att is None:
+        left = tuple(getattr(impl, "sliding_window", None) or (-1, -1))[0]
+        att = _DENSE[size] = PagedAttention(
+            num_query_heads=impl.num_heads, num_kv_heads=impl.num_kv_heads, max_requests=size[1], token_capacity=slots,
+            dtype=kv_cache.dtype, device=kv_cache.device, max_query_len=T, scale=float(impl.scale),
+            softcap=float(getattr(impl, "logits_soft_cap", None) or 0.0), alibi_slopes=getattr(impl, "alibi_slopes", None),
+            window=left + 1 if left >= 0 else 0)
+    att.bind_kv_paged(kv_cache, table)
+    lens = attn_metadata.seq_lens
+    if lens.dtype != torch.int32 or not lens.is_contiguous():
+        lens = lens.to(torch.int32).contiguous()
+    q = query[: n * T].reshape(n, T, impl.num_heads, 128)
+    if output.is_contiguous() and output.dtype == kv_cache.dtype and q.dtype == kv_cache.dtype:
+        att.forward(q, lens, out=output[: n * T].view(q.shape))
+    else:
+        output[: n * T].copy_(att.forward(q.to(kv_cache.dtype), lens).reshape(output[: n * T].shape))
+    STATS["library_dense_steps"] = STATS.get("library_dense_steps", 0) + 1
+    return output
+
+
 def pq_or_dense_forward(original, impl, layer, query, key, value, kv_cache, attn_metadata, output=None, **extra):
     if not should_pq_decode(attn_metadata) or output is None:
+        if output is not None and dense_enabled() and should_dense_decode(impl, kv_cache, attn_metadata):
+            return run_dense_decode(impl, layer, query, key, value, kv_cache, attn_metadata, output)
         STATS["dense_steps"] += 1
         return original(impl, layer, query, key, value, kv_cache, attn_metadata, output=output, **extra)
     try:
