@@ -88,7 +88,7 @@ static PagedArgs paged_args(const pqhsa_paged_params* p) {
   a.scale_log2 = p->scale * kLog2e;
   a.softcap = p->softcap;
   a.cap_log2 = p->softcap * kLog2e;
-  a.cap_in = p->softcap > 0.f ? p->scale / p->softcap : 0.f;
+  a.cap_in = p->softcap > 0.f ? 2.f * kLog2e * p->scale / p->softcap : 0.f;
   a.slopes = p->alibi_slopes;
   a.window = p->window; a.sinks = p->sink_tokens;
   a.seq_lens = p->seq_lens; a.first_key = p->first_key; a.query_pos = p->query_pos;
