@@ -18,6 +18,8 @@
 // Keys that no row may see are not read at all: their rows in shared memory are filled with zeros, so whatever a page
 // holds there (NaN included) stays out.  A key that only some rows of the step see takes part with p = 0 for the
 // others, and its value row is multiplied only where p is not 0.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace pqhsa {
@@ -236,6 +238,15 @@ __device__ __forceinline__ float4 tile_piece(const float* tile, int key, int ele
   return *reinterpret_cast<const float4*>(tile + key * kD + (((elem >> 2) ^ (key & 7)) << 2));
 }
 
+__device__ __forceinline__ ulonglong2 tile_pairs(const float* tile, int key, int elem) {
+  return *reinterpret_cast<const ulonglong2*>(tile + key * kD + (((elem >> 2) ^ (key & 7)) << 2));
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {  // of two floats each
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 template <int ROWS, int STAGES, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const PagedArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -331,32 +342,34 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const Paged
       const float* kt = ring + st * kStage;
       const float* vt = kt + kKeys * kD;
       float s[ROWS];
+      uint64_t s2[ROWS];  // sums of even and of odd dimensions: two multiply-adds an instruction
 #pragma unroll
-      for (int i = 0; i < ROWS; ++i) s[i] = 0.f;
+      for (int i = 0; i < ROWS; ++i) s2[i] = 0ull;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {  // 32 dimensions of a quarter, 4 at a time, each quarter in its own order (banks)
         const int d = quarter * 32 + ((j ^ (2 * quarter)) & 7) * 4;
-        const float4 kv = tile_piece(kt, key, d);
+        const ulonglong2 kv = tile_pairs(kt, key, d);
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-          const float4 qv = *reinterpret_cast<const float4*>(q_s + i * kD + d);
-          s[i] = fmaf(kv.x, qv.x, fmaf(kv.y, qv.y, fmaf(kv.z, qv.z, fmaf(kv.w, qv.w, s[i]))));
+          const ulonglong2 qv = *reinterpret_cast<const ulonglong2*>(q_s + i * kD + d);
+          s2[i] = fma_pair(kv.y, qv.y, fma_pair(kv.x, qv.x, s2[i]));
         }
       }
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
+        s[i] = __uint_as_float((uint32_t)s2[i]) + __uint_as_float((uint32_t)(s2[i] >> 32));
         s[i] += __shfl_xor_sync(0xffffffffu, s[i], 8);
         s[i] += __shfl_xor_sync(0xffffffffu, s[i], 16);
       }
       const int pos = pos_s[warp][st][key];
       const unsigned flags = (unsigned)seen_s[warp][st];
-      const bool here = (flags >> key) & 1u;
       float own[OWN];
       bool raise = false;
 #pragma unroll
       for (int i = 0; i < OWN; ++i) {
         const float dot = quarter == 0 ? s[4 * i] : quarter == 1 ? s[4 * i + 1] : quarter == 2 ? s[4 * i + 2] : s[4 * i + 3];
-        own[i] = here && paged_sees(c.g, a, pos, p_at[i]) ? paged_score(a, dot, slope[i], p_at[i] - pos) : kNegInf;
+        own[i] = paged_score(a, dot, slope[i], p_at[i] - pos);
+        if (flags != 0xffu && !(((flags >> key) & 1u) != 0u && paged_sees(c.g, a, pos, p_at[i]))) own[i] = kNegInf;
         raise |= own[i] > m[i] + kLazy;
       }
       if (a.scores != nullptr) {
@@ -394,26 +407,29 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const Paged
         p_s[(4 * i + quarter) * kKeys + key] = p;
       }
       __syncwarp();
-      const bool guard = (flags >> 16) != 0u;  // a key that only some rows see: its value is multiplied only where p is not 0
+      auto values = [&](auto guard) {  // guard: a key that only some rows see is multiplied only where p is not 0
 #pragma unroll
-      for (int k4 = 0; k4 < kKeys; k4 += 4) {
-        float4 v[4];
+        for (int k4 = 0; k4 < kKeys; k4 += 4) {
+          float4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = tile_piece(vt, k4 + k, lane * 4);
+          for (int k = 0; k < 4; ++k) v[k] = tile_piece(vt, k4 + k, lane * 4);
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-          const float4 p = *reinterpret_cast<const float4*>(p_s + i * kKeys + k4);
-          const float pk[4] = {p.x, p.y, p.z, p.w};
+          for (int i = 0; i < ROWS; ++i) {
+            const float4 p = *reinterpret_cast<const float4*>(p_s + i * kKeys + k4);
+            const float pk[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (guard && pk[k] == 0.f) continue;
-            acc[i][0] = fmaf(pk[k], v[k].x, acc[i][0]);
-            acc[i][1] = fmaf(pk[k], v[k].y, acc[i][1]);
-            acc[i][2] = fmaf(pk[k], v[k].z, acc[i][2]);
-            acc[i][3] = fmaf(pk[k], v[k].w, acc[i][3]);
+            for (int k = 0; k < 4; ++k) {
+              if (guard.value && pk[k] == 0.f) continue;
+              acc[i][0] = fmaf(pk[k], v[k].x, acc[i][0]);
+              acc[i][1] = fmaf(pk[k], v[k].y, acc[i][1]);
+              acc[i][2] = fmaf(pk[k], v[k].z, acc[i][2]);
+              acc[i][3] = fmaf(pk[k], v[k].w, acc[i][3]);
+            }
           }
         }
-      }
+      };
+      if ((flags >> 16) != 0u) values(std::true_type{});
+      else values(std::false_type{});
       __syncwarp();  // the slot may be filled again
     }
     cp_async_wait<0>();
