@@ -101,7 +101,9 @@ static inline cudaError_t paged_launch(void (*kern)(P...), dim3 grid, int thread
 
 // Every kernel here is launched with programmatic stream serialization: it may be placed on the GPU while the one
 // before it in the stream ends.  wait_for_grid comes before its first access to global memory: from there on it sees
-// all that came before.  next_grid lets the kernel behind be placed from now on instead of at this one's end.
+// all that came before.  (Inputs are read with ordinary loads: the read-only path is for data that does not change
+// while a kernel runs, and this one may have begun before they were written.)  next_grid lets the kernel behind be
+// placed from now on instead of at this one's end.
 __device__ __forceinline__ void wait_for_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void next_grid() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -113,7 +115,7 @@ __device__ __forceinline__ int64_t paged_offset(const PagedArgs& a, int r, int h
   if (a.block_table != nullptr) {
     const int b = t / a.block_size;
     row = t - b * a.block_size;
-    const int32_t e = __ldg(a.block_table + (int64_t)r * a.max_blocks + b);
+    const int32_t e = a.block_table[(int64_t)r * a.max_blocks + b];
     if (e < 0 || e >= a.num_blocks) return -1;
     blk = e;
   }
@@ -130,9 +132,9 @@ struct PagedGeom {
 };
 __device__ __forceinline__ PagedGeom paged_geom(const PagedArgs& a, int r) {
   PagedGeom g;
-  g.n = min(max(__ldg(a.seq_lens + r), 0), a.limit);
-  g.first = a.first_key != nullptr ? max(__ldg(a.first_key + r), 0) : 0;
-  g.p_last = a.query_pos != nullptr ? max(__ldg(a.query_pos + r), -1) : g.n - 1;
+  g.n = min(max(a.seq_lens[r], 0), a.limit);
+  g.first = a.first_key != nullptr ? max(a.first_key[r], 0) : 0;
+  g.p_last = a.query_pos != nullptr ? max(a.query_pos[r], -1) : g.n - 1;
   g.p_first = g.p_last - (a.T - 1);
   const int tl = a.tile_log2, up = (1 << tl) - 1;
   const int end = (g.n + up) >> tl;
@@ -141,7 +143,7 @@ __device__ __forceinline__ PagedGeom paged_geom(const PagedArgs& a, int r) {
     const int lo = min(g.first, g.n);
     g.b0 = lo >> tl;
     if (a.window > 0) {
-      const int w = min(max(lo, g.p_first - a.window + 1), g.n);       // first slot of the window
+      const int w = (int)min(max((long long)lo, (long long)g.p_first - a.window + 1), (long long)g.n);  // first slot of the window
       const int s = min(a.sinks, w - lo);                              // sink slots in front of it
       g.a0 = lo >> tl;
       g.na = s > 0 ? ((lo + s + up) >> tl) - g.a0 : 0;

@@ -116,8 +116,8 @@ int pqhsa_paged_attention(const pqhsa_paged_params* p, void* stream) {
   if (int rc = check_rows(p, p->q, p->q_stride_request, p->q_stride_token, p->q_stride_head, "q")) return rc;
   if (int rc = check_rows(p, p->out, p->out_stride_request, p->out_stride_token, p->out_stride_head, "out")) return rc;
   if (p->key_pos != nullptr && p->query_pos == nullptr) return set_error(PQHSA_E_NULL, "key_pos needs query_pos");
-  if (!isfinite(p->scale) || !isfinite(p->softcap) || p->softcap < 0.f)
-    return set_error(PQHSA_E_SHAPE, "scale must be finite and softcap finite and non-negative");
+  if (!isfinite(p->scale) || !isfinite(p->softcap) || p->softcap < 0.f || !isfinite(paged_args(p).cap_in))
+    return set_error(PQHSA_E_SHAPE, "scale must be finite, softcap finite, non-negative and not vanishing against scale");
   if (!p->workspace || ((uintptr_t)p->workspace & 255))
     return set_error(PQHSA_E_WORKSPACE, "workspace missing or not 256-byte aligned");
   if (sm_count() > kPagedMaxCtas) return set_error(PQHSA_E_CAPACITY, "more than %d SMs", kPagedMaxCtas);

@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const Paged
         int pos = -1;
         if (slot < c.g.n) {
           off = paged_offset(a, c.r, h, slot);
-          pos = kpos != nullptr ? __ldg(kpos + slot) : slot;
+          pos = kpos != nullptr ? max(kpos[slot], -1) : slot;
         }
         const PagedSight v = paged_sight(c.g, a, off >= 0, pos);
         const unsigned seen = __ballot_sync(0xffffffffu, v.any) & 0xffu, mixed = __ballot_sync(0xffffffffu, v.any && !v.all) & 0xffu;
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const Paged
       const int row = i / (kD / 4), d = i % (kD / 4) * 4, full = row0 + row;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (row < rows)
-        v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)c.r * a.q_sr + (int64_t)h * a.G * a.q_sh + a.q_row(full) + d));
+        v = *(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + (int64_t)c.r * a.q_sr + (int64_t)h * a.G * a.q_sh + a.q_row(full) + d));
       *reinterpret_cast<float4*>(q_s + row * kD + d) = v;
     }
     float slope[OWN], m[OWN], l[OWN], acc[ROWS][4];
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) paged_attend_kernel(const Paged
       const int full = row0 + 4 * i + quarter;
       const bool live = 4 * i + quarter < rows;
       p_at[i] = live ? c.g.p_first + a.token_of(full) : -1;
-      slope[i] = live && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + a.head_of(full)) : 0.f;
+      slope[i] = live && a.slopes != nullptr ? kLog2e * a.slopes[h * a.G + a.head_of(full)] : 0.f;
       m[i] = kFloor;
       l[i] = 0.f;
     }
@@ -578,16 +578,17 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
     n_pos = slot;
     const bool there = slot < ahead.g.n;
     if (!there) n_pos = n_entry = -1;
-    if (a.key_pos != nullptr && there) n_pos = __ldg(a.key_pos + ((int64_t)ahead.r * a.H + ahead.h) * a.cap + slot);
+    if (a.key_pos != nullptr && there) n_pos = a.key_pos[((int64_t)ahead.r * a.H + ahead.h) * a.cap + slot];
     if (a.block_table != nullptr) {
       const int b = (unsigned)slot / (unsigned)a.block_size;
       n_row = slot - b * a.block_size;
-      if (there) n_entry = __ldg(a.block_table + (int64_t)ahead.r * a.max_blocks + b);
+      if (there) n_entry = a.block_table[(int64_t)ahead.r * a.max_blocks + b];
     }
   };
   auto load = [&](int st) {  // `ahead` is still in the tile's stream
     if (more) {
       const PagedGeom& g = ahead.g;
+      n_pos = max(n_pos, -1);  // not in fetch, which must not wait for what it asks for
       const bool page = n_entry >= 0 && n_entry < a.num_blocks;
       const PagedSight v = paged_sight(g, a, page, n_pos);
       const unsigned seen = __ballot_sync(0xffffffffu, v.any) & 0xffffu, mixed = __ballot_sync(0xffffffffu, v.any && !v.all) << 16;
@@ -637,8 +638,8 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
         const E* src = base + a.q_row(full) + 2 * t4;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
-          qf[nb][kk][0] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
-          qf[nb][kk][1] = row < rows ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
+          qf[nb][kk][0] = row < rows ? *(reinterpret_cast<const uint32_t*>(src + kk * 16)) : 0u;
+          qf[nb][kk][1] = row < rows ? *(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8)) : 0u;
         }
       }
     } else {
@@ -646,7 +647,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
         const int row = i >> 4, piece = i & 15, full = row0 + row;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (row < rows)
-          v = __ldg(reinterpret_cast<const uint4*>(base + a.q_row(full)) + piece);
+          v = *(reinterpret_cast<const uint4*>(base + a.q_row(full)) + piece);
         *reinterpret_cast<uint4*>(q_s + row * 256 + ((piece ^ (row & 7)) << 4)) = v;
       }
       __syncthreads();
@@ -676,7 +677,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
         m[nb][j] = kFloor;
         l[nb][j] = 0.f;
         p_at[nb][j] = row < rows ? c.g.p_first + a.token_of(full) : -1;
-        slope[nb][j] = SHAPED && row < rows && a.slopes != nullptr ? kLog2e * __ldg(a.slopes + h * a.G + a.head_of(full)) : 0.f;
+        slope[nb][j] = SHAPED && row < rows && a.slopes != nullptr ? kLog2e * a.slopes[h * a.G + a.head_of(full)] : 0.f;
       }
 #pragma unroll
       for (int db = 0; db < 8; ++db)
@@ -909,7 +910,8 @@ static int launch_mma(const PagedArgs& a, cudaStream_t st) {
 // thread.  The rows of a key are added in row order by one thread: no atomics, the same bits every run.
 constexpr int kMassThreads = 256;
 __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArgs a) {
-  // a.groups is 1 here: one stream per KV head
+  // a.groups is 1 here: one stream per KV head.  The shares need only what was there before the attention kernel, which
+  // let this one be placed after it had waited for it.
   PagedCursor c;
   PagedShares sh;
   if (!paged_locate(a, gridDim.x, blockIdx.x, kMassThreads / 32, sh, c)) return;

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
   const int64_t stream = blockIdx.y;
   const int r = blockIdx.y / a.H;
   wait_for_grid();
-  const int n = min(max(__ldg(a.seq_lens + r), 0), a.limit), K = e.budget;
+  const int n = min(max(a.seq_lens[r], 0), a.limit), K = e.budget;
   const float* mass = a.mass + stream * a.cap;
   const int32_t* pos = a.key_pos + stream * a.cap;
   float* new_mass = e.new_mass + stream * a.cap;
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
     if (rank == 0 && tid == 0) *count = 0;
     return;
   }
-  const int old = (int)max((long long)__ldg(a.query_pos + r) - e.recent, -2147483648LL);  // a position above it is recent
+  const int old = (int)max((long long)a.query_pos[r] - e.recent, -2147483648LL);  // a position above it is recent
   const int share = ((n + ranks - 1) / ranks + 127) / 128 * 128;
   const int lo = min(rank * share, n), hi = min(lo + share, n);
   // Keys of slots i .. i + 3 (i a multiple of 4 from lo on); 0, which no slot has, past the share.  Sweeps ask for
@@ -107,13 +107,13 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
     m = make_float4(0.f, 0.f, 0.f, 0.f);
     p = make_int4(0, 0, 0, 0);
     if (wide && i + 4 <= hi) {
-      m = __ldg(reinterpret_cast<const float4*>(mass + i));
-      p = __ldg(reinterpret_cast<const int4*>(pos + i));
+      m = *reinterpret_cast<const float4*>(mass + i);
+      p = *reinterpret_cast<const int4*>(pos + i);
     } else {
-      if (i < hi) m.x = __ldg(mass + i), p.x = __ldg(pos + i);
-      if (i + 1 < hi) m.y = __ldg(mass + i + 1), p.y = __ldg(pos + i + 1);
-      if (i + 2 < hi) m.z = __ldg(mass + i + 2), p.z = __ldg(pos + i + 2);
-      if (i + 3 < hi) m.w = __ldg(mass + i + 3), p.w = __ldg(pos + i + 3);
+      if (i < hi) m.x = mass[i], p.x = pos[i];
+      if (i + 1 < hi) m.y = mass[i + 1], p.y = pos[i + 1];
+      if (i + 2 < hi) m.z = mass[i + 2], p.z = pos[i + 2];
+      if (i + 3 < hi) m.w = mass[i + 3], p.w = pos[i + 3];
     }
   };
   auto make = [&](int i, const float4& m, const int4& p) {
@@ -136,8 +136,8 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
       if (apart_pos) *reinterpret_cast<int4*>(new_pos + i) = p;
     } else {
       for (int q = i; q < min(i + 4, to); ++q) {
-        if (apart) new_mass[q] = __ldg(mass + q);
-        if (apart_pos) new_pos[q] = __ldg(pos + q);
+        if (apart) new_mass[q] = mass[q];
+        if (apart_pos) new_pos[q] = pos[q];
       }
     }
   };
@@ -355,9 +355,9 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(const PagedArgs a, c
     const int64_t stream = item / per;
     const int first = (int)(item - stream * per) * kMoves;
     const int32_t* count = e.scratch + stream * (2 * (int64_t)e.budget + 8);
-    if (first + lane < __ldg(count)) {
-      dst = __ldg(count + 8 + first + lane);
-      src = __ldg(count + 8 + e.budget + first + lane);
+    if (first + lane < *count) {
+      dst = count[8 + first + lane];
+      src = count[8 + e.budget + first + lane];
     }
   };
   fetch(w);
@@ -432,7 +432,7 @@ int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaS
 // negative length marks an idle request; rows that do not fit the request's slots, or whose page is missing, are
 // dropped.
 template <typename E>
-__global__ void __launch_bounds__(256) paged_append_kernel(const PagedArgs a, const E* __restrict__ k, const E* __restrict__ v,
+__global__ void __launch_bounds__(256) paged_append_kernel(const PagedArgs a, const E* k, const E* v,
                                                            int32_t* new_lens) {
   const int r = blockIdx.x, lane = threadIdx.x & 31;
   wait_for_grid();

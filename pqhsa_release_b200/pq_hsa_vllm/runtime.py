@@ -355,7 +355,7 @@ def should_dense_decode(impl, kv_cache, attn_metadata) -> bool:
     if kv_cache.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         return reject("dense_dtype")
     left, right = tuple(getattr(impl, "sliding_window", None) or (-1, -1))
-    if right > 0 or getattr(impl, "sinks", None) is not None:
+    if right > 0 or getattr(impl, "sinks", None) is not None or getattr(impl, "kv_sharing_target_layer_name", None) is not None:
         return reject("dense_scores")
     return True
 
