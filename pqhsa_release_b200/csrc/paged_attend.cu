@@ -918,37 +918,58 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArg
   int x = sh.x;
   const int x_end = sh.x_end;
   const int quads = a.tile_log2 - 2;  // log2 of the quads of keys in a tile
+  __shared__ float z_s[kPagedMaxRows];
+  const bool wide = (a.cap & 3) == 0 && ((uintptr_t)a.mass & 15) == 0;
   wait_for_grid();  // scores and row sums are there
   while (true) {
     const int count = min(c.g.tiles - c.tile, x_end - x);
     const int64_t stream = (int64_t)c.r * a.H + c.h;
+    const float* scores = a.scores + stream * a.R * a.score_stride;
+    float* mass = a.mass + stream * a.cap;
+    __syncthreads();  // z_s of the stream before has been read
+    for (int row = threadIdx.x; row < a.R; row += kMassThreads) {
+      const float z = __ldcg(a.row_lse2 + stream * a.R + row);
+      z_s[row] = z == kNegInf ? -kNegInf : z;  // a row that sees no key adds 2^(-inf - inf) = 0
+    }
+    __syncthreads();
     for (int i = threadIdx.x; i < count << quads; i += kMassThreads) {
       const int slot = (paged_tile(c.g, c.tile + (i >> quads)) << a.tile_log2) + ((i & ((1 << quads) - 1)) << 2);
       if (slot >= c.g.n) continue;
-      float w[4] = {0.f, 0.f, 0.f, 0.f}, old[4];
-      float* to = a.mass + stream * a.cap + slot;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) old[j] = slot + j < c.g.n ? to[j] : 0.f;
-      for (int row0 = 0; row0 < a.R; row0 += 4) {
-        float4 s[4];
-        float z[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = min(row0 + j, a.R - 1);
-          s[j] = __ldcg(reinterpret_cast<const float4*>(a.scores + (stream * a.R + row) * a.score_stride + slot));
-          z[j] = row0 + j < a.R ? __ldcg(a.row_lse2 + stream * a.R + row) : -kNegInf;  // 2^(s - inf) = 0: a row that is not there
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[0] += s[j].x == kNegInf ? 0.f : ex2(s[j].x - z[j]);
-          w[1] += s[j].y == kNegInf ? 0.f : ex2(s[j].y - z[j]);
-          w[2] += s[j].z == kNegInf ? 0.f : ex2(s[j].z - z[j]);
-          w[3] += s[j].w == kNegInf ? 0.f : ex2(s[j].w - z[j]);
-        }
+      const bool four = slot + 4 <= c.g.n;
+      float4 old = make_float4(0.f, 0.f, 0.f, 0.f), w = old;
+      if (four && wide) {
+        old = *reinterpret_cast<const float4*>(mass + slot);
+      } else {
+        old.x = mass[slot];
+        if (slot + 1 < c.g.n) old.y = mass[slot + 1];
+        if (slot + 2 < c.g.n) old.z = mass[slot + 2];
+        if (four) old.w = mass[slot + 3];
       }
+      const float* from = scores + slot;
+      auto add = [&](const float4& s, float z) {
+        w.x += ex2(s.x - z);
+        w.y += ex2(s.y - z);
+        w.z += ex2(s.z - z);
+        w.w += ex2(s.w - z);
+      };
+      int row = 0;
+      for (; row + 4 <= a.R; row += 4) {
+        float4 s[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (slot + j < c.g.n && w[j] != 0.f) to[j] = old[j] + w[j];  // keys no row saw are left as they were
+        for (int j = 0; j < 4; ++j, from += a.score_stride) s[j] = __ldcg(reinterpret_cast<const float4*>(from));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) add(s[j], z_s[row + j]);
+      }
+      for (; row < a.R; ++row, from += a.score_stride) add(__ldcg(reinterpret_cast<const float4*>(from)), z_s[row]);
+      // keys that no row saw, whose weight is 0, are left as they were
+      if (four && wide && w.x != 0.f && w.y != 0.f && w.z != 0.f && w.w != 0.f) {
+        *reinterpret_cast<float4*>(mass + slot) = make_float4(old.x + w.x, old.y + w.y, old.z + w.z, old.w + w.w);
+      } else {
+        if (w.x != 0.f) mass[slot] = old.x + w.x;
+        if (w.y != 0.f && slot + 1 < c.g.n) mass[slot + 1] = old.y + w.y;
+        if (w.z != 0.f && slot + 2 < c.g.n) mass[slot + 2] = old.z + w.z;
+        if (w.w != 0.f && four) mass[slot + 3] = old.w + w.w;
+      }
     }
     x += count;
     if (x >= x_end) return;
