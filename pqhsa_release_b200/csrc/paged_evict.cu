@@ -29,11 +29,12 @@ constexpr int kEvShare = 49152;   // most keys a CTA keeps in shared memory (192
 constexpr int kEvAhead = 4;
 template <typename E> constexpr int kEvMoves = 16 / (int)sizeof(E);  // moves of a warp at a time: 4 KB of rows in its registers
 
-// Order-preserving key, +0 and -0 alike, NaN as -inf; positions below `sinks` or above `old` are kept before all others.
-__device__ __forceinline__ uint32_t evict_key(int sinks, int old, float mass, int pos) {
-  const int u = __float_as_int(mass != mass ? kNegInf : mass + 0.f);
+// Order-preserving key, +0 and -0 alike, NaN as -inf (the other operand of fmaxf).  Positions outside sinks ..
+// sinks + free - 1 are kept before all others: one unsigned comparison, true for all with free = 0.
+__device__ __forceinline__ uint32_t evict_key(int sinks, unsigned free, float mass, int pos) {
+  const int u = __float_as_int(fmaxf(mass, kNegInf) + 0.f);
   const uint32_t k = (uint32_t)(u ^ ((u >> 31) | (int)0x80000000));  // float_key without a branch
-  return pos < sinks || pos > old ? 0xff800000u : k;                 // the key of +inf
+  return (unsigned)pos - (unsigned)sinks >= free ? 0xff800000u : k;  // the key of +inf
 }
 
 constexpr int kEvBins = 2048;
@@ -97,7 +98,8 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
     if (rank == 0 && tid == 0) *count = 0;
     return;
   }
-  const int old = (int)max((long long)a.query_pos[r] - e.recent, -2147483648LL);  // a position above it is recent
+  // positions that are neither sinks nor above query_pos - recent
+  const unsigned open = (unsigned)max((long long)a.query_pos[r] - e.recent - a.sinks + 1, 0LL);
   const int share = ((n + ranks - 1) / ranks + 127) / 128 * 128;
   const int lo = min(rank * share, n), hi = min(lo + share, n);
   // Keys of slots i .. i + 3 (i a multiple of 4 from lo on); 0, which no slot has, past the share.  Sweeps ask for
@@ -117,8 +119,8 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
     }
   };
   auto make = [&](int i, const float4& m, const int4& p) {
-    return make_uint4(i < hi ? evict_key(a.sinks, old, m.x, p.x) : 0u, i + 1 < hi ? evict_key(a.sinks, old, m.y, p.y) : 0u,
-                      i + 2 < hi ? evict_key(a.sinks, old, m.z, p.z) : 0u, i + 3 < hi ? evict_key(a.sinks, old, m.w, p.w) : 0u);
+    return make_uint4(i < hi ? evict_key(a.sinks, open, m.x, p.x) : 0u, i + 1 < hi ? evict_key(a.sinks, open, m.y, p.y) : 0u,
+                      i + 2 < hi ? evict_key(a.sinks, open, m.z, p.z) : 0u, i + 3 < hi ? evict_key(a.sinks, open, m.w, p.w) : 0u);
   };
   // What slots below the budget hold if they stay; the moves write over the others.
   const bool wide_source = ((K & 3) | ((uintptr_t)e.source & 15)) == 0;
@@ -148,6 +150,11 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
     fetch(i, m, p);
     return make(i, m, p);
   };
+  auto key1 = [&](int i) {
+    if (i >= hi) return 0u;
+    if constexpr (RESIDENT) return keys_s[i - lo];
+    return evict_key(a.sinks, open, mass[i], pos[i]);
+  };
   for (int i = tid; i < 2 * kEvBins; i += kEvThreads) sh.hist[i / kEvBins][i % kEvBins] = 0u;
   if (tid == 0) {
     sh.prefix = 0u;
@@ -172,31 +179,34 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
       infs += k == key_inf;
       if (k != key_zero && k != key_inf) atomicAdd(&hist[(k >> shift) & digit_mask], 1u);
     };
-    for (int b = lo + 4 * tid; b < hi; b += 4 * kEvThreads * kEvAhead) {
-      uint4 k[kEvAhead];
+    constexpr int kStep = 4 * kEvThreads;
+    for (int b = lo + 4 * tid; b < hi; b += kStep * kEvAhead) {
       if (pass == 0) {
         float4 m[kEvAhead];
         int4 p[kEvAhead];
 #pragma unroll
-        for (int u = 0; u < kEvAhead; ++u) fetch(b + 4 * kEvThreads * u, m[u], p[u]);
+        for (int u = 0; u < kEvAhead; ++u) fetch(b + kStep * u, m[u], p[u]);
 #pragma unroll
         for (int u = 0; u < kEvAhead; ++u) {
-          k[u] = make(b + 4 * kEvThreads * u, m[u], p[u]);
-          stay(b + 4 * kEvThreads * u, m[u], p[u]);
+          const int i = b + kStep * u;
+          if (i >= hi) break;
+          const uint4 k = i + 4 <= hi ? make_uint4(evict_key(a.sinks, open, m[u].x, p[u].x), evict_key(a.sinks, open, m[u].y, p[u].y),
+                                                   evict_key(a.sinks, open, m[u].z, p[u].z), evict_key(a.sinks, open, m[u].w, p[u].w))
+                                      : make(i, m[u], p[u]);
+          if constexpr (RESIDENT) *reinterpret_cast<uint4*>(keys_s + (i - lo)) = k;
+          if (i < K) stay(i, m[u], p[u]);
+          tally(k.x); tally(k.y); tally(k.z); tally(k.w);  // slots past the end count below all that are there
         }
       } else {
+        uint4 k[kEvAhead];
 #pragma unroll
-        for (int u = 0; u < kEvAhead; ++u) k[u] = key4(b + 4 * kEvThreads * u);
-      }
+        for (int u = 0; u < kEvAhead; ++u) k[u] = key4(b + kStep * u);
 #pragma unroll
-      for (int u = 0; u < kEvAhead; ++u) {
-        if constexpr (RESIDENT) {
-          const int i = b + 4 * kEvThreads * u;
-          if (pass == 0 && i < hi) *reinterpret_cast<uint4*>(keys_s + (i - lo)) = k[u];
+        for (int u = 0; u < kEvAhead; ++u) {
+          if (b + kStep * u >= hi) break;
+          if ((k[u].x & mask) != prefix && (k[u].y & mask) != prefix && (k[u].z & mask) != prefix && (k[u].w & mask) != prefix) continue;
+          tally(k[u].x); tally(k[u].y); tally(k[u].z); tally(k[u].w);
         }
-        if (pass > 0 && (k[u].x & mask) != prefix && (k[u].y & mask) != prefix && (k[u].z & mask) != prefix && (k[u].w & mask) != prefix)
-          continue;
-        tally(k[u].x); tally(k[u].y); tally(k[u].z); tally(k[u].w);
       }
     }
     zeros = __reduce_add_sync(0xffffffffu, zeros);
@@ -286,52 +296,28 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
   const int ties = mine.y + mine.w;
   const bool some = tied < take && take < tied + ties;  // in one warp of the cluster at most the ties are told apart
   const uint32_t least = tied >= take ? T + 1u : T;     // smallest key that stays (T is below the largest 32-bit number)
-  uint4 next = key4(begin + 4 * lane);
-  for (int g = begin; g < end; g += 128) {
-    const int i = g + 4 * lane;
-    const uint4 k4 = next;
-    next = key4(i + 128);
-    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-    int tie = 0;
+  const unsigned below = (1u << lane) - 1u;
+  // 32 slots at a time, so that what a warp adds to a list is one run of words
+#pragma unroll 4
+  for (int g = begin; g < end; g += 32) {
+    const int i = g + lane;
+    const uint32_t k = key1(i);
+    bool keep = k >= least;
     if (some) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tie += k[q] == T;
-      int incl = tie;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
-      }
-      const int all = __shfl_sync(0xffffffffu, incl, 31);
-      tie = tied + incl - tie;  // rank of this lane's first
-      tied += all;
+      const unsigned same = __ballot_sync(0xffffffffu, k == T);
+      if (k == T) keep = tied + __popc(same & below) < take;
+      tied += __popc(same);
     }
-    unsigned hole = 0u, late = 0u;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      bool keep = k[q] >= least;
-      if (some && k[q] == T) keep = tie++ < take;
-      const bool low = i + q < K;
-      hole |= (!keep && low && i + q < end ? 1u : 0u) << q;
-      late |= (keep && !low ? 1u : 0u) << q;
+    if (g < K) {
+      const unsigned hole = __ballot_sync(0xffffffffu, i < min(K, end) && !keep);
+      if ((hole >> lane) & 1u) holes[at_hole + __popc(hole & below)] = i;
+      at_hole += __popc(hole);
     }
-    const int own = __popc(hole) | __popc(late) << 16;
-    if (!__any_sync(0xffffffffu, own != 0)) continue;
-    int incl = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+    if (g + 32 > K) {
+      const unsigned late = __ballot_sync(0xffffffffu, i >= K && keep);
+      if ((late >> lane) & 1u) lates[at_late + __popc(late & below)] = i;
+      at_late += __popc(late);
     }
-    const int all = __shfl_sync(0xffffffffu, incl, 31);
-    int ah = at_hole + ((incl - own) & 0xffff), al = at_late + ((incl - own) >> 16);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if ((hole >> q) & 1u) holes[ah++] = i + q;
-      if ((late >> q) & 1u) lates[al++] = i + q;
-    }
-    at_hole += all & 0xffff;
-    at_late += all >> 16;
   }
   if (rank == ranks - 1 && tid == kEvThreads - 1) *count = at_late;  // the last range ends with all of them
   if (ranks > 1) cluster.barrier_wait();  // no CTA ends while another may read its shared memory
