@@ -422,3 +422,114 @@ def test_evict_long(n, budget):
     mass[torch.rand(2, 1, cap, generator=g) < 0.5] = 0.125
     pos = torch.arange(cap, dtype=torch.int32).repeat(2, 1, 1)
     evict_case([n, n // 2], 1, BF, 64, "heads", budget, 64, 4, mass.cuda(), pos.cuda(), [n - 1, n // 2 - 1], True)
+
+
+def test_evict_past_what_shared_memory_holds():
+    """More slots than the eight CTAs of a cluster keep: every sweep makes the keys again."""
+    n, budget = 400_001, 300
+    g = torch.Generator().manual_seed(1)
+    cap = Cache([n], 1, BF, 64, "heads").cap
+    mass = torch.exp(torch.randn(1, 1, cap, generator=g))
+    mass[0, 0, ::3] = 20.0
+    pos = torch.arange(cap, dtype=torch.int32).repeat(1, 1, 1)
+    evict_case([n], 1, BF, 64, "heads", budget, 16, 4, mass.cuda(), pos.cuda(), [n - 1], True)
+
+
+# ---- extremes and refusals --------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+def test_extreme_windows_and_positions(dtype):
+    top = 2**31 - 1
+    cache = Cache([50, 20], 1, dtype, 16, "heads")
+    pos = torch.full((2, 1, cache.cap), top, dtype=torch.int32, device="cuda")
+    pos[:, :, ::2] = torch.arange(cache.cap // 2, dtype=torch.int32, device="cuda") * 3
+    pos[0, 0, 1], pos[0, 0, 3] = -(2**31), top - 1
+    for window, sinks in ((top, 0), (1, 7), (2, top), (0, 0)):
+        run(cache, 2, 3, key_pos=pos, query_pos=[top, 30], window=window, sink_tokens=sinks)
+    run(cache, 2, 2, window=top, sink_tokens=top)
+    run(cache, 2, 1, first=[top, -5])
+    run(cache, 2, 2, key_pos=pos, query_pos=[-(2**31), -1])
+
+
+def test_forward_refusals():
+    cache = Cache([10, 10], 2, BF, 16, "rows")
+    att = layer(cache, 4, 2)
+    q = torch.zeros(2, 8, D, dtype=BF, device="cuda")
+    lens = cache.seq_lens
+    pos = torch.zeros(2, 2, cache.cap, dtype=torch.int32, device="cuda")
+    mass = torch.zeros(2, 2, cache.cap, device="cuda")
+    ok = dict(q=q, seq_lens=lens)
+    bad = [
+        dict(q=q.float()), dict(q=q.cpu()), dict(q=q[:, :7]), dict(q=q[..., :64]), dict(q=torch.zeros(3, 8, D, dtype=BF, device="cuda")),
+        dict(q=torch.zeros(2, 3, 8, D, dtype=BF, device="cuda")), dict(q=torch.zeros(2, 8, D + 4, dtype=BF, device="cuda")[..., 4:]),
+        dict(q=torch.zeros(2, 8, 2 * D, dtype=BF, device="cuda")[..., ::2]), dict(q=q[0]),
+        dict(seq_lens=lens.long()), dict(seq_lens=lens[:1]), dict(seq_lens=lens.cpu()), dict(out=torch.empty(2, 8, D, device="cuda")),
+        dict(out=torch.empty(2, 4, D, dtype=BF, device="cuda")), dict(lse=torch.empty(2, 4, device="cuda")),
+        dict(lse=torch.empty(2, 8, dtype=BF, device="cuda")), dict(first_key=lens.long()), dict(key_pos=pos), dict(key_pos=pos.long(), query_pos=lens),
+        dict(key_pos=pos[:, :, :-1], query_pos=lens), dict(mass=mass.double()), dict(mass=mass[:1]), dict(mass=mass[:, :1]),
+    ]
+    att.forward(**ok)
+    for kw in bad:
+        with pytest.raises(ValueError):
+            att.forward(**{**ok, **kw})
+    free = PagedAttention(num_query_heads=8, num_kv_heads=2, max_requests=2, token_capacity=16, dtype=BF, device="cuda")
+    with pytest.raises(RuntimeError, match="bind"):
+        free.forward(q, lens)
+    for kv, table in [(cache.kv.float(), cache.table), (cache.kv, cache.table.long()), (cache.kv[:1], cache.table), (cache.kv[..., :64], cache.table),
+                      (cache.kv[0, 0], cache.table), (cache.kv, cache.table[:, :0]), (cache.kv[:, :, :, :1], cache.table)]:
+        with pytest.raises(ValueError):
+            free.bind_kv_paged(kv, table)
+    with pytest.raises(ValueError):
+        free.bind_kv_contiguous(cache.kv[0], cache.kv[0])
+    k = torch.zeros(2, 2, D, dtype=BF, device="cuda")
+    for kw in (dict(keys=k.float()), dict(values=k[:1]), dict(keys=k[:, :1], values=k[:, :1]), dict(new_lens=lens.long()), dict(mass=mass[:1])):
+        with pytest.raises(ValueError):
+            att.append(**{**dict(keys=k, values=k, seq_lens=lens), **kw})
+    ev = dict(seq_lens=lens, mass=mass, key_pos=pos, query_pos=lens, budget=8)
+    for kw in (dict(budget=0), dict(recent=9), dict(recent=-1), dict(mass=mass.double()), dict(key_pos=pos[:1]), dict(query_pos=lens.long()),
+               dict(source=torch.zeros(2, 2, 7, dtype=torch.int32, device="cuda")), dict(new_mass=mass[:1]), dict(new_lens=lens[:1])):
+        with pytest.raises(ValueError):
+            att.evict(**{**ev, **kw})
+    torch.cuda.synchronize()
+
+
+def test_no_requests_and_fewer_than_the_layer_was_made_for():
+    cache = Cache([100, 200, 30], 2, BF, 16, "rows")
+    att = layer(cache, 4)
+    q = queries(cache, 4, 1)
+    assert att.forward(q[:0], cache.seq_lens[:0]).shape == (0, 1, 8, D)
+    want = ref.attend(cache, q)
+    for b in (3, 1, 2, 3):  # workspaces of different sizes in turn
+        mass = torch.zeros(3, 2, cache.cap, device="cuda")
+        out = att.forward(q[:b], cache.seq_lens[:b], mass=mass if b % 2 else None)
+        check(out, None, tuple(x[:b] for x in want))
+
+
+def test_two_graphs_with_weights_at_once():
+    cache = Cache([2000, 700], 2, BF, 16, "heads")
+    att = layer(cache, 4)
+    qs = [queries(cache, 4, 1, s) for s in (1, 2)]
+    masses = [torch.zeros(2, 2, cache.cap, device="cuda") for _ in qs]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in qs]
+    for q, m in zip(qs, masses):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(att.forward(q, cache.seq_lens, mass=m))
+        graphs.append(g)
+    for m in masses:
+        m.zero_()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for q, m, o in zip(qs, masses, outs):
+        check(o, None, ref.attend(cache, q))
+        one = torch.zeros_like(m)
+        att.forward(q, cache.seq_lens, mass=one)
+        ten = torch.zeros_like(m)
+        for _ in range(10):
+            ten += one
+        assert torch.equal(m, ten)
