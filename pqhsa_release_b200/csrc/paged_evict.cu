@@ -11,10 +11,10 @@
 // Two launches.  The selection is one thread block cluster per stream: the CTAs keep the keys of their share of the
 // slots in shared memory (read once), find the budget-th largest in three passes of 11, 11 and 10 bits over a histogram
 // that is summed through distributed shared memory, then number the holes and the kept slots behind the budget in slot order
-// and write both lists.  The moves go over the whole GPU, eight to a warp (four in fp32), all their loads in flight before the stores:
+// and write both lists.  The moves go over the whole GPU, four to a warp, all their loads in flight before the stores:
 // they are the bytes of the operator (4 rows a move against 8 bytes a slot for the selection).  One B200, 32 streams from
-// 131072 slots down to 16384: selection 33 us (34 MB read; three passes with a cluster barrier each), moves 89 us
-// (470 MB, 5.3 TB/s with rows of 256 bytes in random order).
+// 131072 slots down to 16384: selection 28 us (34 MB read; three passes with a cluster barrier each), moves 90 us
+// (470 MB, 5.2 TB/s with rows of 256 bytes in random order; eight to a warp and four CTAs to an SM 4 us more).
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -27,7 +27,8 @@ constexpr int kEvThreads = 1024;
 constexpr int kEvWarps = kEvThreads / 32;
 constexpr int kEvShare = 49152;   // most keys a CTA keeps in shared memory (192 KB)
 constexpr int kEvAhead = 4;
-template <typename E> constexpr int kEvMoves = 16 / (int)sizeof(E);  // moves of a warp at a time: 4 KB of rows in its registers
+constexpr int kEvMoves = 4;       // moves of a warp at a time
+template <typename E> constexpr int kEvMoveCtas = sizeof(E) == 2 ? 5 : 4;  // CTAs of them on an SM: as many as hold their rows in registers
 
 // Order-preserving key, +0 and -0 alike, NaN as -inf (the other operand of fmaxf).  Positions outside sinks ..
 // sinks + free - 1 are kept before all others: one unsigned comparison, true for all with free = 0.
@@ -325,8 +326,7 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
 
 // The moves of an item (kEvMoves of a stream): where lane j moves a row from and to, asked for one item ahead.
 template <typename E>
-__global__ void __launch_bounds__(256, 4) evict_move_kernel(const PagedArgs a, const PagedEvict e, int per) {
-  constexpr int kMoves = kEvMoves<E>;
+__global__ void __launch_bounds__(256, kEvMoveCtas<E>) evict_move_kernel(const PagedArgs a, const PagedEvict e, int per) {
   const int lane = threadIdx.x & 31;
   const long long warps = (long long)gridDim.x * (blockDim.x >> 5), items = (long long)a.B * a.H * per;
   E* kb = static_cast<E*>(const_cast<void*>(a.k_base));
@@ -337,9 +337,9 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(const PagedArgs a, c
   int dst = -1, src = -1;
   auto fetch = [&](long long item) {
     dst = -1;
-    if (item >= items || lane >= kMoves) return;
+    if (item >= items || lane >= kEvMoves) return;
     const int64_t stream = item / per;
-    const int first = (int)(item - stream * per) * kMoves;
+    const int first = (int)(item - stream * per) * kEvMoves;
     const int32_t* count = e.scratch + stream * (2 * (int64_t)e.budget + 8);
     if (first + lane < *count) {
       dst = count[8 + first + lane];
@@ -363,9 +363,9 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(const PagedArgs a, c
     }
     fetch(w + warps);
     const E* base = lane < 16 ? kb : vb;
-    uint4 row[kMoves][half];
+    uint4 row[kEvMoves][half];
 #pragma unroll
-    for (int j = 0; j < kMoves; ++j) {
+    for (int j = 0; j < kEvMoves; ++j) {
       const int64_t f = __shfl_sync(0xffffffffu, from, j);
       if (__shfl_sync(0xffffffffu, to, j) >= 0) {
 #pragma unroll
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(256, 4) evict_move_kernel(const PagedArgs a, c
       e.new_pos[stream * a.cap + d0] = pos;
     }
 #pragma unroll
-    for (int j = 0; j < kMoves; ++j) {
+    for (int j = 0; j < kEvMoves; ++j) {
       const int64_t t = __shfl_sync(0xffffffffu, to, j);
       if (t >= 0) {
 #pragma unroll
@@ -405,8 +405,8 @@ int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaS
     return check_launch("evict_select shared memory");
   if (paged_launch(kern, dim3(ranks, a.B * a.H), kEvThreads, smem, st, ranks, a, e) != cudaSuccess) return check_launch("evict_select");
   const int most = e.budget < a.limit ? (e.budget < a.limit - e.budget ? e.budget : a.limit - e.budget) : 0;
-  const int at_once = dtype == PQHSA_F32 ? kEvMoves<float> : kEvMoves<__half>, per = (most + at_once - 1) / at_once;
-  const long long want = ((long long)a.B * a.H * per + 7) / 8 + 1, cap = (long long)sm_count() * 4;
+  const int per = (most + kEvMoves - 1) / kEvMoves;
+  const long long want = ((long long)a.B * a.H * per + 7) / 8 + 1, cap = (long long)sm_count() * (dtype == PQHSA_F32 ? kEvMoveCtas<float> : kEvMoveCtas<__half>);
   const unsigned grid = (unsigned)(want < cap ? want : cap);
   PQHSA_DISPATCH_E(dtype, {
     if (paged_launch(evict_move_kernel<E>, dim3(grid), 256, 0, st, 0, a, e, per > 0 ? per : 1) != cudaSuccess) return check_launch("evict_move");
