@@ -328,18 +328,18 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
 template <typename E>
 __global__ void __launch_bounds__(256, kEvMoveCtas<E>) evict_move_kernel(const PagedArgs a, const PagedEvict e, int per) {
   const int lane = threadIdx.x & 31;
-  const long long warps = (long long)gridDim.x * (blockDim.x >> 5), items = (long long)a.B * a.H * per;
+  const int warps = gridDim.x * (blockDim.x >> 5), items = a.B * a.H * per;  // 31 bits: the host bounds requests x heads x slots
   E* kb = static_cast<E*>(const_cast<void*>(a.k_base));
   E* vb = static_cast<E*>(const_cast<void*>(a.v_base));
   constexpr int half = sizeof(E) / 2;  // 16-byte pieces of a row for each of 16 lanes
-  long long w = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  int w = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   wait_for_grid();
   int dst = -1, src = -1;
-  auto fetch = [&](long long item) {
+  auto fetch = [&](int item) {
     dst = -1;
     if (item >= items || lane >= kEvMoves) return;
-    const int64_t stream = item / per;
-    const int first = (int)(item - stream * per) * kEvMoves;
+    const int st = item / per, first = (item - st * per) * kEvMoves;
+    const int64_t stream = st;
     const int32_t* count = e.scratch + stream * (2 * (int64_t)e.budget + 8);
     if (first + lane < *count) {
       dst = count[8 + first + lane];
@@ -348,9 +348,9 @@ __global__ void __launch_bounds__(256, kEvMoveCtas<E>) evict_move_kernel(const P
   };
   fetch(w);
   for (; w < items; w += warps) {
-    const int64_t stream = w / per;
-    const int r = (int)(stream / a.H), h = (int)(stream % a.H);
-    int64_t from = -1, to = -1;
+    const int st = w / per, r = st / a.H, h = st - r * a.H;
+    const int64_t stream = st;
+    int64_t from = 0, to = -1;
     float mass = 0.f;
     int pos = 0;
     const int d0 = dst, s0 = src;
@@ -359,18 +359,17 @@ __global__ void __launch_bounds__(256, kEvMoveCtas<E>) evict_move_kernel(const P
       to = paged_offset(a, r, h, d0);
       mass = a.mass[stream * a.cap + s0];
       pos = a.key_pos[stream * a.cap + s0];
-      if (from < 0) to = -1;
+      if (from < 0) from = 0, to = -1;
     }
     fetch(w + warps);
     const E* base = lane < 16 ? kb : vb;
     uint4 row[kEvMoves][half];
 #pragma unroll
     for (int j = 0; j < kEvMoves; ++j) {
+      // a row that does not move is read from the cache's first place, so that no load waits behind a branch
       const int64_t f = __shfl_sync(0xffffffffu, from, j);
-      if (__shfl_sync(0xffffffffu, to, j) >= 0) {
 #pragma unroll
-        for (int p = 0; p < half; ++p) row[j][p] = __ldcs(reinterpret_cast<const uint4*>(base + f) + (lane & 15) + 16 * p);
-      }
+      for (int p = 0; p < half; ++p) row[j][p] = __ldcs(reinterpret_cast<const uint4*>(base + f) + (lane & 15) + 16 * p);
     }
     if (d0 >= 0) {
       e.source[stream * e.budget + d0] = s0;
