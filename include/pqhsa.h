@@ -470,17 +470,17 @@ size_t pqhsa_paged_workspace_bytes(const pqhsa_paged_params* p);
 int pqhsa_paged_attention(const pqhsa_paged_params* p, void* stream);
 
 /* Write new rows k, v (strides q_stride_* of p, over KV heads) of query_len tokens per request to slots
- * seq_lens[r] .. + query_len - 1, their positions (the slots themselves without query_pos) to key_pos and 0 to mass (where given); new_lens[r] = seq_lens[r] +
- * query_len (may be seq_lens itself).  A negative length is an idle request and stays; rows past the request's slots
- * or on missing pages are dropped. */
+ * seq_lens[r] .. + query_len - 1, their positions (the slots themselves without query_pos) to key_pos and 0 to mass
+ * (where given); new_lens[r] = seq_lens[r] + query_len (may be seq_lens itself).  A negative length is an idle request
+ * and stays; rows past the request's slots or on missing pages are dropped. */
 int pqhsa_paged_append(const pqhsa_paged_params* p, const void* k, const void* v, int32_t* new_lens, void* stream);
 
 /* Keep, per request and KV head, the `budget` slots of the largest mass - the sink_tokens first and the `recent` last
- * positions (x > query_pos[r] - recent) before all others, NaN behind all, ties to the lower slot - in slots
- * 0 .. budget - 1: a kept slot below the budget stays, the i-th of the other slots below it (ascending) takes over the
- * i-th kept slot behind it: its K and V rows in place, its mass and position in new_mass / new_pos (may be mass /
- * key_pos themselves).  source int32 [requests, kv_heads, budget] receives the slot each slot now holds (-1 past the
- * request's keys), new_lens[r] = min(seq_lens[r], budget) (may be seq_lens itself).  scratch: int32 [requests,
+ * positions (x < sink_tokens, x > query_pos[r] - recent) before all others, NaN behind all, ties to the lower slot -
+ * in slots 0 .. budget - 1: a kept slot below the budget stays, the i-th of the other slots below it (ascending) takes
+ * over the i-th kept slot behind it: its K and V rows in place, its mass and position in new_mass / new_pos (may be
+ * mass / key_pos themselves).  source int32 [requests, kv_heads, budget] receives the slot each slot now holds (-1 past
+ * the request's keys), new_lens[r] = min(seq_lens[r], budget) (may be seq_lens itself).  scratch: int32 [requests,
  * kv_heads, 2 * budget + 8].  requests * kv_heads <= 65535.  Slots behind the new length are left as they were.
  * Needs mass, key_pos and query_pos; the pages must belong to one request each. */
 int pqhsa_paged_evict(const pqhsa_paged_params* p, int32_t budget, int32_t recent, int32_t* new_lens, float* new_mass,

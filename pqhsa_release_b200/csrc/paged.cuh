@@ -24,7 +24,7 @@ struct PagedArgs {
   int32_t groups;              // passes over a KV head's keys: ceil(R / kPagedGroupRows)
   int32_t cap;                 // row stride of key_pos / mass / scores
   int32_t limit;               // slots a request can have: min(cap, what its block-table row addresses)
-  float scale_log2, softcap, cap_log2, cap_in;  // see score() in paged_attend.cu
+  float scale_log2, softcap, cap_log2, cap_in;  // cap_log2 = softcap log2(e), cap_in = 2 log2(e) scale / softcap
   const float* slopes;
   int32_t window, sinks;
   const int32_t* seq_lens;

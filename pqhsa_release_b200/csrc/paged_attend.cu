@@ -8,7 +8,7 @@
 // keys for more than 32 rows).  One pass with a running maximum and sum per row, in the base-2 domain and in fp32.
 //
 // Split: the key tiles of all (request, KV head, pass) streams form one sequence; a persistent grid of one CTA per SM
-// takes equal contiguous shares of it (paged.cuh).  Inside a CTA the tiles of a stream go to the warps in turn, each
+// takes shares of it, equal ones or whole numbers of CTAs to a stream (paged.cuh).  Inside a CTA the tiles of a stream go to the warps in turn, each
 // with a ring of tiles in shared memory filled by 16-byte asynchronous copies; the warps' states are merged in shared
 // memory where a stream (or the share) ends.  A stream that lies in one share is finished there; of one that several
 // CTAs share (at most two of a CTA's streams: its first and its last), each writes (max, sum, acc) as it gets there
@@ -36,13 +36,19 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t smem, const void* gmem
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(take ? 16 : 0) : "memory");
 }
 
-// cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap)), x = scale dot, in log2 units: two approximations of 2^-22 on
-// a value of 1, so off by 2^-22 of the cap, where the sum behind a score is off by more (130 roundings of its terms).
-// Five instructions against some twenty-five of tanhf; infinities end at the cap, NaN stays.
+// cap tanh(x / cap), x = scale dot, in log2 units, of z = 2 log2(e) x / cap.
+//
+// |x| >= cap / 16: cap - 2 cap / (1 + 2^z), two approximations of 2^-22 on a value of 1: off by 2^-18 of the score at
+// most, where the sum behind it is off by more (130 roundings of its terms).  Below, where the difference would cancel
+// (all scores, with a cap that is large against them): x (1 - u^2 / 3 + 2 u^4 / 15), u = x / cap, whose next term is
+// 17 u^6 / 315 < 2^-28.  Eleven instructions against some twenty-five of tanhf; infinities end at the cap, NaN stays.
 __device__ __forceinline__ float capped(const PagedArgs& a, float dot) {
+  constexpr float kZ2 = 1.f / (4.f * kLog2e * kLog2e);  // u^2 of z^2
+  const float z = dot * a.cap_in, z2 = z * z;
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(dot * a.cap_in)));
-  return fmaf(-2.f * a.cap_log2, r, a.cap_log2);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(z)));
+  const float x = dot * a.scale_log2, small = fmaf(x * z2, fmaf(z2, kZ2 * kZ2 * 2.f / 15.f, -kZ2 / 3.f), x);
+  return z2 < 1.f / (256.f * kZ2) ? small : fmaf(-2.f * a.cap_log2, r, a.cap_log2);
 }
 // score in log2 units of a dot product; p - x is the distance of the key
 __device__ __forceinline__ float paged_score(const PagedArgs& a, float dot, float slope_log2, int distance) {

@@ -533,3 +533,9 @@ def test_two_graphs_with_weights_at_once():
         for _ in range(10):
             ten += one
         assert torch.equal(m, ten)
+
+
+@pytest.mark.parametrize("dtype,T", [(BF, 1), (HF, 4), (F32, 1)], ids=["bf16", "fp16x4", "fp32"])
+@pytest.mark.parametrize("softcap", [0.02, 1.0, 300.0, 1e5, 1e9, 3e38])
+def test_caps_small_and_large_against_the_scores(dtype, T, softcap):
+    run(Cache([300, 5, 700], 2, dtype, 16, "heads"), 4, T, softcap=softcap, mass=True)
