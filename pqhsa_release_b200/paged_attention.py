@@ -238,6 +238,7 @@ class PagedAttention:
         p.q, p.out = self._rows_at(q, "q"), self._rows_at(out, "out")
         even = q.is_contiguous() and out.is_contiguous()
         if not even or shape != self._forward_shape:
+            self._forward_shape = None  # what follows may refuse the call with the block half set
             p.requests, p.query_len = self._tokens(shape, "q", self.Hq)
             p.q_stride_request, p.q_stride_token, p.q_stride_head = self._strides_of(q, "q")
             p.out_stride_request, p.out_stride_token, p.out_stride_head = self._strides_of(out, "out")
@@ -277,6 +278,7 @@ class PagedAttention:
             raise ValueError("keys and values must have the same shape")
         even = keys.is_contiguous() and values.is_contiguous()
         if not even or shape != self._append_shape:
+            self._append_shape = None
             p.requests, p.query_len = self._tokens(shape, "keys", self.H)
             s = self._strides_of(keys, "keys")
             if self._strides_of(values, "values") != s:

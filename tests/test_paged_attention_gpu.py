@@ -539,3 +539,24 @@ def test_two_graphs_with_weights_at_once():
 @pytest.mark.parametrize("softcap", [0.02, 1.0, 300.0, 1e5, 1e9, 3e38])
 def test_caps_small_and_large_against_the_scores(dtype, T, softcap):
     run(Cache([300, 5, 700], 2, dtype, 16, "heads"), 4, T, softcap=softcap, mass=True)
+
+
+def test_a_refused_call_leaves_the_next_one_alone():
+    cache = Cache([60, 33, 90], 2, BF, 16, "heads")
+    q = queries(cache, 4, 1).squeeze(1)
+    att = layer(cache, 4, 1)
+    want = att.forward(q, cache.seq_lens)
+    odd = torch.zeros(1, 8, 2 * D, dtype=BF, device="cuda")[:, :, ::2]  # elements of a row apart
+    with pytest.raises(ValueError, match="contiguous"):
+        att.forward(odd, cache.seq_lens[:1])
+    assert torch.equal(att.forward(q, cache.seq_lens), want)
+    k = torch.randn(3, 2, D, device="cuda").to(BF)
+    lens = cache.seq_lens - 1  # the last rows are written again
+    kept = cache.kv.clone()
+    att.append(k, k, lens.clone())
+    first = cache.kv.clone()
+    cache.kv.copy_(kept)
+    with pytest.raises(ValueError, match="contiguous"):
+        att.append(odd[:, :2], odd[:, :2], lens[:1].clone())
+    att.append(k, k, lens.clone())
+    assert torch.equal(cache.kv, first)
