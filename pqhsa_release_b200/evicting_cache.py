@@ -26,7 +26,7 @@ class EvictingCacheAdapter:
     def __init__(self, *, num_query_heads: int, num_kv_heads: int, budget: int, interval: int = 256, sink_tokens: int = 4,
                  recent: int = 128, scale: float | None = None, softcap: float = 0.0,
                  alibi_slopes: torch.Tensor | None = None, window: int = 0) -> None:
-        if num_kv_heads < 1 or num_query_heads % num_kv_heads != 0:
+        if num_kv_heads < 1 or num_query_heads < 1 or num_query_heads % num_kv_heads != 0:
             raise ValueError("GQA requires num_query_heads % num_kv_heads == 0")
         if budget < 1 or interval < 1 or sink_tokens < 0 or recent < 0 or sink_tokens + recent > budget:
             raise ValueError("need budget >= 1, interval >= 1 and sink_tokens + recent <= budget")
@@ -73,6 +73,7 @@ class EvictingCacheAdapter:
         self.lens = torch.full((B,), S, dtype=torch.int32, device=dev)
         self.query_pos = torch.full((B,), S - 1, dtype=torch.int32, device=dev)
         self.length = self.position = S
+        self.evictions = 0
         if queries is not None:
             W, step = queries.shape[2], self.attention.max_query_len
             for lo in range(0, W, step):  # a few tokens at a time, each seeing what lies before it
@@ -108,6 +109,9 @@ class EvictingCacheAdapter:
         keys, values = _squeeze_decode_token(keys, "keys"), _squeeze_decode_token(values, "values")
         if keys.shape != (self.keys.shape[0], self.num_kv_heads, _lib.HEAD_DIM) or values.shape != keys.shape:
             raise ValueError(f"keys and values must be [{self.keys.shape[0]}, {self.num_kv_heads}, 128]")
+        for x in (keys, values):  # before anything is counted or moved
+            if x.dtype != self.keys.dtype or x.device != self.keys.device:
+                raise ValueError(f"keys and values must be {self.keys.dtype} tensors on {self.keys.device}, got {x.dtype} on {x.device}")
         if self.length >= self.budget + self.interval:
             self._evict()
         self.query_pos.add_(1)

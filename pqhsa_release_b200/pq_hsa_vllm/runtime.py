@@ -28,7 +28,9 @@ STATS: dict[str, int] = {"pq_steps": 0, "dense_steps": 0, "builds": 0, "flushes"
                          "restores": 0, "evictions": 0, "kv_writes": 0}
 _REJECTS: dict[str, int] = {}
 _LAYERS: dict[int, Any] = {}  # id(layer) -> PagedBatchEngine
-_DENSE: dict[tuple, Any] = {}  # (id(layer), requests, query tokens, slots, dtype) -> PagedAttention, kept for captured graphs
+# (id of the layer's implementation, requests, query tokens, slots, dtype, device) -> (the implementation, held so that no
+# other can have its id, its PagedAttention); kept for captured graphs
+_DENSE: dict[tuple, Any] = {}
 
 
 def reject(reason: str) -> bool:
@@ -368,24 +370,27 @@ def run_dense_decode(impl, layer, query, key, value, kv_cache, attn_metadata, ou
     from ..paged_kv import kv_cache_dims
 
     T, n = int(attn_metadata.max_query_len), int(attn_metadata.seq_lens.shape[0])
-    write_step_kv(key, value, kv_cache, attn_metadata)
     table = attn_metadata.block_table[:n]
     if table.dtype != torch.int32 or not table.is_contiguous():
         table = table.to(torch.int32).contiguous()
     slots = int(table.shape[1]) * kv_cache_dims(kv_cache)[0]
-    size = (id(layer), 1 << (n - 1).bit_length(), T, slots, kv_cache.dtype)
-    att = _DENSE.get(size)
-    if att is None:
+    size = (id(impl), 1 << (n - 1).bit_length(), T, slots, kv_cache.dtype, kv_cache.device)
+    if size not in _DENSE:
         left = tuple(getattr(impl, "sliding_window", None) or (-1, -1))[0]
-        att = _DENSE[size] = PagedAttention(
+        _DENSE[size] = impl, PagedAttention(
             num_query_heads=impl.num_heads, num_kv_heads=impl.num_kv_heads, max_requests=size[1], token_capacity=slots,
             dtype=kv_cache.dtype, device=kv_cache.device, max_query_len=T, scale=float(impl.scale),
             softcap=float(getattr(impl, "logits_soft_cap", None) or 0.0), alibi_slopes=getattr(impl, "alibi_slopes", None),
             window=left + 1 if left >= 0 else 0)
+    att = _DENSE[size][1]
     att.bind_kv_paged(kv_cache, table)
     lens = attn_metadata.seq_lens
     if lens.dtype != torch.int32 or not lens.is_contiguous():
         lens = lens.to(torch.int32).contiguous()
+    if kv_cache.dim() == 5:  # the older pages, see write_step_kv; by lengths, so that a padded batch's idle requests (length 0) write nothing
+        k, v = (x[: n * T].reshape(n, T, impl.num_kv_heads, 128).to(kv_cache.dtype).contiguous() for x in (key, value))
+        att.append(k, v, lens - T)
+        STATS["kv_writes"] += 1
     q = query[: n * T].reshape(n, T, impl.num_heads, 128)
     if output.is_contiguous() and output.dtype == kv_cache.dtype and q.dtype == kv_cache.dtype:
         att.forward(q, lens, out=output[: n * T].view(q.shape))

@@ -222,3 +222,78 @@ def test_hook_serves_short_requests_with_the_dense_kernel(layout, T, monkeypatch
     runtime.pq_or_dense_forward(original, impl, layer, q, k, v, cache.kv, md2, output=out)
     assert len(calls) == 2 and runtime.STATS["dense_steps"] == 2
     runtime.reset()
+
+
+def test_a_refused_append_changes_nothing():
+    from pqhsa_release_b200 import EvictingCacheAdapter
+
+    ad = EvictingCacheAdapter(num_query_heads=8, num_kv_heads=2, budget=32, interval=8, sink_tokens=2, recent=4)
+    k = torch.randn(1, 2, 40, D, device="cuda").to(BF)
+    ad.build_cache(k[:, :, :39], k[:, :, :39])
+    ad.append(k[:, :, 39], k[:, :, 39])  # full: the next append evicts first
+    before = [x.clone() for x in (ad.keys, ad.values, ad.positions, ad.weights, ad.lens, ad.query_pos)]
+    for bad in (k[:, :, 0].float(), k[:, :, 0].cpu()):
+        with pytest.raises(ValueError, match="tensors on"):
+            ad.append(bad, bad)
+        assert (ad.length, ad.position, ad.evictions) == (40, 40, 0)
+        assert all(torch.equal(a, b) for a, b in zip(before, (ad.keys, ad.values, ad.positions, ad.weights, ad.lens, ad.query_pos)))
+    ad.append(k[:, :, 0], k[:, :, 0])
+    assert (ad.length, ad.position, ad.evictions) == (33, 41, 1)
+    ad.build_cache(k[:, :, :10], k[:, :, :10])
+    assert (ad.length, ad.position, ad.evictions) == (10, 10, 0)
+    with pytest.raises(ValueError, match="GQA"):
+        EvictingCacheAdapter(num_query_heads=0, num_kv_heads=2, budget=32, recent=4)
+
+
+def test_hook_keeps_nothing_of_a_layer_that_is_gone(monkeypatch):
+    from pqhsa_release_b200.pq_hsa_vllm import runtime
+
+    for k, v in {"PQ_HSA_BATCH": "1", "PQ_HSA_ENABLE": "1", "PQ_HSA_DENSE": "1", "PQ_HSA_MULTI_QUERY": "0"}.items():
+        monkeypatch.setenv(k, v)
+    runtime.reset()
+    H, G = 2, 4
+    cache = Cache([70, 5, 131], H, BF, 16, "heads")
+    q = torch.randn(3, H * G, D, device="cuda").to(BF)
+    md = metadata(cache, 1)
+    for left in (-1, 3, 20, 50, -1, 9):
+        impl = NS(scale=0.1, num_heads=H * G, num_kv_heads=H, sliding_window=(left, 0 if left >= 0 else -1), logits_soft_cap=0, alibi_slopes=None)
+        layer, out = object(), torch.zeros_like(q)  # often at the address of the one before
+        kv = torch.zeros(3, H, D, dtype=BF, device="cuda")
+        runtime.pq_or_dense_forward(None, impl, layer, q, kv, kv, cache.kv, md, output=out)
+        o, _, _, tol, _ = ref.attend(cache, q.view(3, 1, H * G, D), scale=0.1, window=left + 1)
+        assert ((out.view(3, 1, H * G, D).double() - o).abs() <= tol).all(), left
+        del impl, layer
+    runtime.reset()
+
+
+@pytest.mark.parametrize("layout", ["rows", "heads"])
+def test_hook_with_a_padded_batch(layout, monkeypatch):
+    """Two idle requests (length 0, slot -1) and two rows behind the batch, as a captured step of a fixed size has them."""
+    from pqhsa_release_b200.pq_hsa_vllm import runtime
+
+    for k, v in {"PQ_HSA_BATCH": "1", "PQ_HSA_ENABLE": "1", "PQ_HSA_DENSE": "1", "PQ_HSA_MULTI_QUERY": "0"}.items():
+        monkeypatch.setenv(k, v)
+    runtime.reset()
+    H, G = 2, 4
+    cache = Cache([70, 0, 131, 0], H, BF, 16, layout)
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(6, H * G, D, generator=g).to(BF).cuda()
+    k, v = torch.randn(2, 6, H, D, generator=g).to(BF).cuda()
+    want = cache.kv.clone()
+    for r, n in ((0, 70), (2, 131)):
+        for h in range(H):
+            cache.put(r, h, n - 1, k[r, h], v[r, h])
+    want, cache.kv[:] = cache.kv.clone(), want
+    if layout == "heads":  # written before the forward
+        cache.kv[:] = want
+    slots = [int(cache.table[r, (n - 1) // 16]) * 16 + (n - 1) % 16 if n else -1 for r, n in enumerate(cache.lens)] + [-1, -1]
+    md = NS(use_cascade=False, max_query_len=1, num_actual_tokens=4, seq_lens=cache.seq_lens, seq_lens_cpu=cache.seq_lens.cpu(),
+            max_seq_len=131, block_table=cache.table, slot_mapping=torch.tensor(slots, device="cuda"))
+    impl = NS(scale=0.1, num_heads=H * G, num_kv_heads=H, sliding_window=(-1, -1), logits_soft_cap=0, alibi_slopes=None)
+    out = torch.full_like(q, 7.0)
+    runtime.pq_or_dense_forward(None, impl, object(), q, k, v, cache.kv, md, output=out)
+    assert torch.equal(cache.kv, want)
+    o, _, _, tol, _ = ref.attend(cache, q[:4].view(4, 1, H * G, D), scale=0.1)
+    assert ((out[:4].view(4, 1, H * G, D).double() - o).abs() <= tol).all()
+    assert bool((out[4:] == 7.0).all()) and not bool(out[[1, 3]].any())
+    runtime.reset()
