@@ -391,8 +391,8 @@ __global__ void __launch_bounds__(256, kEvMoveCtas<E>) evict_move_kernel(const P
 
 int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaStream_t st) {
   // CTAs per stream: enough that a share fits shared memory twice over, and with few streams enough to use the GPU.
-  // The histograms of a cluster cross its network: on 32 streams of 128K slots 4 CTAs of 1024 threads take 33 us, 8 of
-  // 512 take 47 (2 CTAs of an SM ask for 128 KB a pass); on 8 streams of 4352 slots one CTA takes 13 us, two 15.
+  // The histograms of a cluster cross its network: on 32 streams of 128K slots 8 CTAs of 512 threads took 47 us where
+  // 4 of 1024 took 33, now 28 (2 CTAs of an SM ask for 128 KB a pass); on 8 streams of 4352 slots one CTA takes 13 us, two 15.
   int ranks = 1;
   while (ranks < 8 && (a.limit > ranks * 32768 || (a.limit > ranks * 8192 && a.B * a.H * ranks * 2 <= sm_count()))) ranks *= 2;
   const int share = ((a.limit + ranks - 1) / ranks + 127) / 128 * 128;
