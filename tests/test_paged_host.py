@@ -127,3 +127,27 @@ def test_parameter_block_matches_the_header():
         if len(words) == 2:
             names += [n.strip() for n in words[1].split(",")]
     assert names == [n for n, _ in PagedParams._fields_]
+
+
+def test_hook_takes_only_the_steps_it_can_serve():
+    from types import SimpleNamespace as NS
+
+    from pqhsa_release_b200.pq_hsa_vllm import runtime
+
+    def ask(impl=(), md=(), kv=None):
+        i = dict(num_heads=8, num_kv_heads=2, sliding_window=(-1, -1), logits_soft_cap=0, alibi_slopes=None)
+        m = dict(use_cascade=False, max_query_len=1, num_actual_tokens=3, seq_lens=torch.tensor([4, 0, 9], dtype=torch.int32))
+        i.update(impl)
+        m.update(md)
+        return runtime.should_dense_decode(NS(**i), torch.zeros(4, 2, 16, 256, dtype=torch.bfloat16) if kv is None else kv, NS(**m))
+
+    assert ask() and ask(impl=dict(sliding_window=(39, 0))) and ask(md=dict(max_query_len=2, num_actual_tokens=6))
+    assert ask(kv=torch.zeros(2, 4, 16, 2, 128))
+    assert not runtime.should_dense_decode(NS(num_heads=8, num_kv_heads=2), torch.zeros(4, 2, 16, 256), None)
+    for impl in (dict(num_heads=64), dict(num_heads=9), dict(num_kv_heads=4), dict(attn_type="encoder_only"), dict(sliding_window=(5, 5)),
+                 dict(sinks=torch.zeros(8)), dict(kv_sharing_target_layer_name="a"), dict(dcp_world_size=2)):
+        assert not ask(impl=impl), impl
+    for md in (dict(use_cascade=True), dict(seq_lens=None), dict(max_query_len=9, num_actual_tokens=27), dict(num_actual_tokens=2)):
+        assert not ask(md=md), md
+    for kv in (torch.zeros(4, 2, 16, 128, dtype=torch.bfloat16), torch.zeros(4, 2, 16, 256, dtype=torch.uint8), torch.zeros(4, 2, 256)):
+        assert not ask(kv=kv), tuple(kv.shape)
