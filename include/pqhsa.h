@@ -482,6 +482,8 @@ int pqhsa_paged_append(const pqhsa_paged_params* p, const void* k, const void* v
  * mass / key_pos themselves).  source int32 [requests, kv_heads, budget] receives the slot each slot now holds (-1 past
  * the request's keys), new_lens[r] = min(seq_lens[r], budget) (may be seq_lens itself).  scratch: int32 [requests,
  * kv_heads, 2 * budget + 8].  requests * kv_heads <= 65535.  Slots behind the new length are left as they were.
+ * A slot whose page is not in the cache is neither moved nor moved to: below the budget it stays and takes a place of the
+ * budget (protected keys that then find none go too, highest slots first), behind it it is dropped.
  * Needs mass, key_pos and query_pos; the pages must belong to one request each. */
 int pqhsa_paged_evict(const pqhsa_paged_params* p, int32_t budget, int32_t recent, int32_t* new_lens, float* new_mass,
                       int32_t* new_pos, int32_t* source, int32_t* scratch, void* stream);

@@ -122,6 +122,11 @@ __device__ __forceinline__ int64_t paged_offset(const PagedArgs& a, int r, int h
   return blk * a.stride_block + (int64_t)h * a.stride_head + (int64_t)row * a.stride_row;
 }
 
+// Whether the page of slot t of request r is in the cache.
+__device__ __forceinline__ bool paged_there(const PagedArgs& a, int r, int t) {
+  return a.block_table == nullptr || (unsigned)a.block_table[(int64_t)r * a.max_blocks + t / a.block_size] < (unsigned)a.num_blocks;
+}
+
 // What a request's query tokens can see.  Query token t sits at position p_first + t; a key at position x is visible
 // to position p when first <= x <= p and (no window, or p - x < window, or x - first < sinks).  Slots are positions
 // unless key_pos says otherwise; then every slot has to be looked at, else only the tiles of [first, first + sinks)

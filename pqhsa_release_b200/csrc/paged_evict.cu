@@ -8,6 +8,10 @@
 // lie behind the budget and all targets below it, so the moves need no order among themselves; a key's position moves
 // with it (key_pos), which is what the attention goes by.
 //
+// A slot whose page is not in the cache holds nothing that could be moved, and nothing can be moved to it: below the
+// budget it ranks before all keys (it stays what it is, and the budget has a slot less for others), behind it after all.
+// At least `budget` slots rank before the latter (those below the budget alone are as many), so none of them is kept.
+//
 // Two launches.  The selection is one thread block cluster per stream: the CTAs keep the keys of their share of the
 // slots in shared memory (read once), find the budget-th largest in three passes of 11, 11 and 10 bits over a histogram
 // that is summed through distributed shared memory, then number the holes and the kept slots behind the budget in slot order
@@ -37,6 +41,8 @@ __device__ __forceinline__ uint32_t evict_key(int sinks, unsigned free, float ma
   const uint32_t k = (uint32_t)(u ^ ((u >> 31) | (int)0x80000000));  // float_key without a branch
   return (unsigned)pos - (unsigned)sinks >= free ? 0xff800000u : k;  // the key of +inf
 }
+
+constexpr uint32_t kEvStays = 0xff800001u, kEvGone = 1u;  // keys of slots on missing pages: above that of +inf, below that of -inf
 
 constexpr int kEvBins = 2048;
 struct EvictShared {
@@ -144,24 +150,34 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
       }
     }
   };
-  auto key4 = [&](int i) {
-    if constexpr (RESIDENT) return i < hi ? *reinterpret_cast<const uint4*>(keys_s + (i - lo)) : make_uint4(0u, 0u, 0u, 0u);
-    float4 m;
-    int4 p;
-    fetch(i, m, p);
-    return make(i, m, p);
-  };
-  auto key1 = [&](int i) {
-    if (i >= hi) return 0u;
-    if constexpr (RESIDENT) return keys_s[i - lo];
-    return evict_key(a.sinks, open, mass[i], pos[i]);
-  };
+  // Pages of the share that are not in the cache: rare, so slots are asked for theirs one by one only where there is one.
+  bool gap = false;
+  if (a.block_table != nullptr && lo < hi)
+    for (int b = lo / a.block_size + tid; b <= (hi - 1) / a.block_size; b += kEvThreads)
+      gap |= (unsigned)a.block_table[(int64_t)r * a.max_blocks + b] >= (unsigned)a.num_blocks;
   for (int i = tid; i < 2 * kEvBins; i += kEvThreads) sh.hist[i / kEvBins][i % kEvBins] = 0u;
   if (tid == 0) {
     sh.prefix = 0u;
     sh.remaining = K;
   }
-  __syncthreads();
+  const bool gaps = __syncthreads_or(gap) != 0;
+  auto placed = [&](int i, uint32_t k) { return i >= hi || paged_there(a, r, i) ? k : i < K ? kEvStays : kEvGone; };
+  auto placed4 = [&](int i, const uint4& k) {
+    return gaps ? make_uint4(placed(i, k.x), placed(i + 1, k.y), placed(i + 2, k.z), placed(i + 3, k.w)) : k;
+  };
+  auto key4 = [&](int i) {
+    if constexpr (RESIDENT) return i < hi ? *reinterpret_cast<const uint4*>(keys_s + (i - lo)) : make_uint4(0u, 0u, 0u, 0u);
+    float4 m;
+    int4 p;
+    fetch(i, m, p);
+    return placed4(i, make(i, m, p));
+  };
+  auto key1 = [&](int i) {
+    if (i >= hi) return 0u;
+    if constexpr (RESIDENT) return keys_s[i - lo];
+    const uint32_t k = evict_key(a.sinks, open, mass[i], pos[i]);
+    return gaps ? placed(i, k) : k;
+  };
 
   // The K-th largest key T, and how many of the slots with that key stay.  Keys that many slots share (no weight, and
   // the protected ones) are counted in registers: atomics of a warp to one address would queue up.
@@ -191,9 +207,9 @@ __global__ void __launch_bounds__(kEvThreads, 1) evict_select_kernel(const Paged
         for (int u = 0; u < kEvAhead; ++u) {
           const int i = b + kStep * u;
           if (i >= hi) break;
-          const uint4 k = i + 4 <= hi ? make_uint4(evict_key(a.sinks, open, m[u].x, p[u].x), evict_key(a.sinks, open, m[u].y, p[u].y),
-                                                   evict_key(a.sinks, open, m[u].z, p[u].z), evict_key(a.sinks, open, m[u].w, p[u].w))
-                                      : make(i, m[u], p[u]);
+          const uint4 k = placed4(i, i + 4 <= hi ? make_uint4(evict_key(a.sinks, open, m[u].x, p[u].x), evict_key(a.sinks, open, m[u].y, p[u].y),
+                                                              evict_key(a.sinks, open, m[u].z, p[u].z), evict_key(a.sinks, open, m[u].w, p[u].w))
+                                                 : make(i, m[u], p[u]));
           if constexpr (RESIDENT) *reinterpret_cast<uint4*>(keys_s + (i - lo)) = k;
           if (i < K) stay(i, m[u], p[u]);
           tally(k.x); tally(k.y); tally(k.z); tally(k.w);  // slots past the end count below all that are there
@@ -359,7 +375,7 @@ __global__ void __launch_bounds__(256, kEvMoveCtas<E>) evict_move_kernel(const P
       to = paged_offset(a, r, h, d0);
       mass = a.mass[stream * a.cap + s0];
       pos = a.key_pos[stream * a.cap + s0];
-      if (from < 0) from = 0, to = -1;
+      if (from < 0) from = 0, to = -1;  // the selection moves only between pages that are there: bounds, should the table change
     }
     fetch(w + warps);
     const E* base = lane < 16 ? kb : vb;

@@ -300,7 +300,8 @@ class PagedAttention:
         first ``budget`` slots with as few moves as possible (K and V rows in place; ``mass`` and ``key_pos`` in place
         too unless ``new_mass`` / ``new_pos`` are given).  Returns ``new_lens``, ``seq_lens`` itself if not given.
         ``source`` int32 ``[B, Hkv, budget]`` receives the former slot of every kept slot (-1 past the end).  The pages
-        of a request must be its own; whole pages behind the new length may be freed."""
+        of a request must be its own; whole pages behind the new length may be freed.  A slot on a page that the block
+        table does not have is never moved or filled: below the budget it takes one of its places, behind it it goes."""
         if _current_device() != self._index:
             with torch.cuda.device(self._index):
                 return self.evict(seq_lens, mass=mass, key_pos=key_pos, query_pos=query_pos, budget=budget, recent=recent,
