@@ -477,9 +477,19 @@ static int launch_fp32(const PagedArgs& a, cudaStream_t st) {
 // lie (ldmatrix), V the A operand transposed (ldmatrix.trans); P^T gets from the accumulator layout of S^T into the B
 // layout with one 8x8 transpose in registers per 8 keys.  A thread holds the same two query rows of every 8 in S^T and
 // in O^T, so maxima, sums and rescaling need no exchange.  p is rounded to the 16-bit type for the product with V (half
-// a step of a value in 0 .. 2^8; the sum it is divided by keeps 32 bits).  Against one row per m16 (P V with 16 rows
+// a step; the sum it is divided by adds them unrounded in 32 bits).  Against one row per m16 (P V with 16 rows
 // of which 4 or 8 are real) this halves the instructions and the accumulators.
+//
+// fp16 has no numbers between 0 and 2^-24, and few bits below 2^-14: with p = 2^(s - m) at most 2^8, thousands of keys some
+// 17 nats below one loud key (a sink) would vanish from the product while the sum counts them.  Its p are therefore
+// 2^(s - m) with m = kBelow under the row's maximum when it is raised, and raised again after 2 more: at most 2^15, a
+// whole half down to 2^-27 of the row's largest weight, off by at most 2^-38 of it further below.  bf16 has the exponents
+// of fp32.
 constexpr int kMKeys = 16;
+template <typename E> constexpr float kBelow = 0.f;
+template <> constexpr float kBelow<__half> = 13.f;
+template <typename E> constexpr float kRaise = kLazy;
+template <> constexpr float kRaise<__half> = 15.f;
 
 template <typename E> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
@@ -750,7 +760,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) raise |= s[nb][j] > m[nb][j & 1] + kLazy;
+        for (int j = 0; j < 4; ++j) raise |= s[nb][j] > m[nb][j & 1] + kRaise<E>;
       if (a.scores != nullptr) {
         const int slot = paged_tile(c.g, c.tile + warp + it * kPWarps) * kMKeys + l4;
         float* dst = a.scores + (((int64_t)c.r * a.H + h) * a.R + row0 + 2 * t4) * a.score_stride + slot;
@@ -769,7 +779,7 @@ __global__ void __launch_bounds__(kPThreads, 1) paged_attend_mma_kernel(const Pa
             float top = fmaxf(s[nb][j], s[nb][j + 2]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float to = fmaxf(m[nb][j], top);
+            const float to = fmaxf(m[nb][j], top - kBelow<E>);
             const float f = ex2(m[nb][j] - to);
             m[nb][j] = to;
             l[nb][j] *= f;
