@@ -962,11 +962,13 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArg
         if (four) old.w = mass[slot + 3];
       }
       const float* from = scores + slot;
+      // a key that the row does not see has no weight of it, not even of a row whose sum is NaN
+      auto weight = [](float s, float z) { return s == kNegInf ? 0.f : ex2(s - z); };
       auto add = [&](const float4& s, float z) {
-        w.x += ex2(s.x - z);
-        w.y += ex2(s.y - z);
-        w.z += ex2(s.z - z);
-        w.w += ex2(s.w - z);
+        w.x += weight(s.x, z);
+        w.y += weight(s.y, z);
+        w.z += weight(s.z, z);
+        w.w += weight(s.w, z);
       };
       int row = 0;
       for (; row + 4 <= a.R; row += 4) {

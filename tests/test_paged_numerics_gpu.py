@@ -47,3 +47,29 @@ def test_keys_far_below_a_loud_one_keep_their_share(dtype, G, T, gap, spread):
     lse = torch.empty(B, T, G, device="cuda")
     out = layer(many, G, T, scale=1.0).forward(q.expand(B, T, G, D).contiguous(), many.seq_lens, lse=lse)
     check(out, lse, tuple(x.expand(B, *x.shape[1:]) if torch.is_tensor(x) else x for x in (o, z, None, tol, ds)))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T", [1, 3])
+def test_a_nan_row_adds_nothing_to_keys_it_does_not_see(dtype, T):
+    """One query head of NaN: the weights of the keys it sees become NaN, those of the keys no row sees stay as they are,
+    in the tiles that hold both: before the document, outside the window, on a missing page, behind an early token."""
+    n, first, window, sinks = 300, 70, 100, 5
+    cache = Cache([n, n], 2, dtype, 16, "heads")
+    q = queries(cache, 4, T)
+    q[0, 0, 1] = math.nan  # the first token of the first request, a head of KV head 0
+    cache.table[:, 14] = -1
+    mass = torch.rand(2, 2, cache.cap, device="cuda")
+    before = mass.clone()
+    att = layer(cache, 4, T, window=window, sink_tokens=sinks)
+    att.forward(q, cache.seq_lens, first_key=torch.tensor([first, first], dtype=torch.int32, device="cuda"), mass=mass)
+    pos = torch.arange(cache.cap, device="cuda")
+    there = (pos // 16 != 14) & (pos < n)
+    by = [there & ref.visible(pos, n - T + t, first, window, sinks) for t in range(T)]
+    for r in range(2):
+        for h in range(2):
+            nan = by[0] if r == 0 and h == 0 else torch.zeros_like(there)
+            seen = torch.stack(by).any(0)
+            assert torch.equal(mass[r, h].isnan(), nan), (r, h)
+            assert torch.equal(mass[r, h][~seen], before[r, h][~seen]), (r, h)
+            assert bool((mass[r, h][seen & ~nan] > before[r, h][seen & ~nan]).all()), (r, h)
