@@ -405,13 +405,16 @@ def run_dense_decode(impl, layer, query, key, value, kv_cache, attn_metadata, ou
 
 
 def pq_or_dense_forward(original, impl, layer, query, key, value, kv_cache, attn_metadata, output=None, **extra):
-    if not should_pq_decode(attn_metadata) or output is None:
-        if output is not None and dense_enabled() and should_dense_decode(impl, kv_cache, attn_metadata):
-            return run_dense_decode(impl, layer, query, key, value, kv_cache, attn_metadata, output)
+    run = None
+    if should_pq_decode(attn_metadata) and output is not None:
+        run = run_pq_decode
+    elif output is not None and dense_enabled() and should_dense_decode(impl, kv_cache, attn_metadata):
+        run = run_dense_decode
+    if run is None:
         STATS["dense_steps"] += 1
         return original(impl, layer, query, key, value, kv_cache, attn_metadata, output=output, **extra)
     try:
-        return run_pq_decode(impl, layer, query, key, value, kv_cache, attn_metadata, output)
+        return run(impl, layer, query, key, value, kv_cache, attn_metadata, output)
     except Exception:
         if os.environ.get("PQ_HSA_FALLBACK", "0") != "1":
             raise

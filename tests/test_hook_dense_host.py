@@ -51,3 +51,24 @@ def test_steps_that_are_not_causal_stay_with_the_engine(taken):
     assert runtime.rejects()["dense_not_causal"] == 1
     assert not step(T=3, md=dict(causal=True)) and not step(T=3) and len(taken) == 2
     assert not step(T=1, md=dict(causal=False)) and len(taken) == 3  # one token sees the same either way
+
+
+@pytest.mark.parametrize("T", [1, 2])
+def test_errors_of_the_dense_path_fall_back_when_asked(T, monkeypatch):
+    """The pages here lie in host memory, which the dense path refuses."""
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        step(T)
+    assert runtime.STATS["fallbacks"] == 0
+    monkeypatch.setenv("PQ_HSA_FALLBACK", "1")
+    assert len(step(T)) == 1
+    assert runtime.STATS["fallbacks"] == 1 and runtime.STATS.get("library_dense_steps", 0) == 0 and runtime.STATS["dense_steps"] == 0
+
+
+def test_an_error_of_the_original_forward_is_not_swallowed(monkeypatch):
+    monkeypatch.setenv("PQ_HSA_FALLBACK", "1")
+
+    def original(*a, **kw):
+        raise KeyError("the engine's own")
+
+    with pytest.raises(KeyError, match="own"):
+        step(original=original)
