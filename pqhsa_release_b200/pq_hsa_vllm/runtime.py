@@ -335,9 +335,10 @@ def dense_enabled() -> bool:
     return os.environ.get("PQ_HSA_DENSE", "0") == "1"
 
 
-def should_dense_decode(impl, kv_cache, attn_metadata) -> bool:
+def should_dense_decode(impl, kv_cache, attn_metadata, extra=()) -> bool:
     """A pure decode step (the same few query tokens for every request) over 128-dimensional heads in a 16- or 32-bit
-    cache; anything else stays with the original forward."""
+    cache; anything else stays with the original forward, and so does a call with more arguments than the path knows
+    (``extra``: a quantised output's scales)."""
     import torch
 
     from ..paged_attention import MAX_GROUP, MAX_QUERY_LEN, MAX_ROWS
@@ -345,6 +346,8 @@ def should_dense_decode(impl, kv_cache, attn_metadata) -> bool:
 
     if attn_metadata is None or getattr(attn_metadata, "use_cascade", False) or getattr(attn_metadata, "seq_lens", None) is None:
         return reject("dense_metadata")
+    if any(v is not None for v in dict(extra).values()):
+        return reject("dense_arguments")
     T, n = int(getattr(attn_metadata, "max_query_len", 0)), int(attn_metadata.seq_lens.shape[0])
     if not 1 <= T <= MAX_QUERY_LEN or n < 1 or int(getattr(attn_metadata, "num_actual_tokens", 0)) != n * T:
         return reject("dense_query_len")
@@ -408,7 +411,7 @@ def pq_or_dense_forward(original, impl, layer, query, key, value, kv_cache, attn
     run = None
     if should_pq_decode(attn_metadata) and output is not None:
         run = run_pq_decode
-    elif output is not None and dense_enabled() and should_dense_decode(impl, kv_cache, attn_metadata):
+    elif output is not None and dense_enabled() and should_dense_decode(impl, kv_cache, attn_metadata, extra):
         run = run_dense_decode
     if run is None:
         STATS["dense_steps"] += 1

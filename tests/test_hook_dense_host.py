@@ -72,3 +72,10 @@ def test_an_error_of_the_original_forward_is_not_swallowed(monkeypatch):
 
     with pytest.raises(KeyError, match="own"):
         step(original=original)
+
+
+def test_arguments_the_dense_path_does_not_know_stay_with_the_engine(taken):
+    scale = torch.ones(1)
+    assert step(extra=dict(output_scale=scale)) == [dict(output_scale=scale)] and not taken
+    assert runtime.rejects()["dense_arguments"] == 1
+    assert not step(extra=dict(output_scale=None, output_block_scale=None)) and len(taken) == 1
