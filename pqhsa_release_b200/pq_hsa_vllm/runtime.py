@@ -364,6 +364,8 @@ def should_dense_decode(impl, kv_cache, attn_metadata, extra=()) -> bool:
     left, right = tuple(getattr(impl, "sliding_window", None) or (-1, -1))
     if right > 0 or getattr(impl, "sinks", None) is not None or getattr(impl, "kv_sharing_target_layer_name", None) is not None:
         return reject("dense_scores")
+    if getattr(impl, "use_irope", False) and getattr(attn_metadata, "local_attn_metadata", None) is not None:  # attention within chunks
+        return reject("dense_scores")
     if int(getattr(impl, "dcp_world_size", 1) or 1) > 1:  # a rank's part of the context, merged with the others' by the engine
         return reject("dense_context_parallel")
     return True

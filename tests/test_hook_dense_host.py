@@ -79,3 +79,10 @@ def test_arguments_the_dense_path_does_not_know_stay_with_the_engine(taken):
     assert step(extra=dict(output_scale=scale)) == [dict(output_scale=scale)] and not taken
     assert runtime.rejects()["dense_arguments"] == 1
     assert not step(extra=dict(output_scale=None, output_block_scale=None)) and len(taken) == 1
+
+
+def test_layers_that_attend_within_chunks_stay_with_the_engine(taken):
+    assert len(step(impl=dict(use_irope=True), md=dict(local_attn_metadata=NS()))) == 1 and not taken
+    assert runtime.rejects()["dense_scores"] == 1
+    assert not step(impl=dict(use_irope=True), md=dict(local_attn_metadata=None)) and not step(md=dict(local_attn_metadata=NS()))
+    assert len(taken) == 2
