@@ -76,14 +76,9 @@ class PagedAttention:
             p.scale, p.softcap, p.window, p.sink_tokens = scale, float(softcap), int(window), int(sink_tokens)
         self.p.alibi_slopes = self.alibi_slopes.data_ptr() if self.alibi_slopes is not None else None
         self._ref, self._append_ref, self._evict_ref = C.byref(self.p), C.byref(self._append_p), C.byref(self._evict_p)
-        self._bytes = []
-        for mass in (None, 1):
-            self.p.mass = mass
-            n = int(_lib.lib.pqhsa_paged_workspace_bytes(self._ref))
-            if n == 0:
-                raise ValueError(_lib.lib.pqhsa_last_error_string().decode("utf-8", "replace"))
-            self._bytes.append(n)
-        self.p.mass = None
+        self._sizes: dict = {}  # (requests, tokens) of a call -> workspace bytes without and with weights
+        if 0 in self._workspace_bytes(self.max_requests, self.max_query_len):
+            raise ValueError(_lib.lib.pqhsa_last_error_string().decode("utf-8", "replace"))
         self._ws: dict = {}
         self._kept: list = []
         self._kv_keepalive = None
@@ -188,6 +183,18 @@ class PagedAttention:
             raise ValueError(f"rows of {name} must be contiguous and 16-byte aligned")
         return s
 
+    def _workspace_bytes(self, requests: int, tokens: int) -> tuple[int, int]:
+        """Workspace of the attention at this size, without and with weights."""
+        got = self._sizes.get((requests, tokens))
+        if got is None:
+            p = _lib.PagedParams.from_buffer_copy(self.p)
+            p.requests, p.query_len, got = requests, tokens, []
+            for mass in (None, 1):
+                p.mass = mass
+                got.append(int(_lib.lib.pqhsa_paged_workspace_bytes(C.byref(p))))
+            got = self._sizes[requests, tokens] = tuple(got)
+        return got
+
     def _scratch(self, kind: str, nbytes: int) -> tuple[int, int]:
         """(address, stream) of this stream's (or this capture's) scratch memory of that kind."""
         stream = _raw_stream(self._index)
@@ -240,6 +247,7 @@ class PagedAttention:
         if not even or shape != self._forward_shape:
             self._forward_shape = None  # what follows may refuse the call with the block half set
             p.requests, p.query_len = self._tokens(shape, "q", self.Hq)
+            self._bytes = self._workspace_bytes(p.requests, p.query_len)
             p.q_stride_request, p.q_stride_token, p.q_stride_head = self._strides_of(q, "q")
             p.out_stride_request, p.out_stride_token, p.out_stride_head = self._strides_of(out, "out")
             self._forward_shape = shape if even else None
