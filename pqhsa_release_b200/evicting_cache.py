@@ -39,14 +39,13 @@ class EvictingCacheAdapter:
         self.evictions = 0
 
     # ---- cache -------------------------------------------------------------------------------------------
-    def _layer(self, keys: torch.Tensor, values: torch.Tensor) -> None:
-        """Bind a layer to these contiguous buffers; positions and weights are [batch, kv_heads, capacity] as they."""
+    def _layer(self, keys: torch.Tensor, values: torch.Tensor, tokens: int = 1) -> PagedAttention:
+        """A layer over these contiguous buffers; positions and weights are [batch, kv_heads, capacity] as they."""
         B, H, cap, _ = keys.shape
-        group = self.num_query_heads // H
-        self.attention = PagedAttention(num_query_heads=self.num_query_heads, num_kv_heads=H, max_requests=B, token_capacity=cap,
-                                        dtype=keys.dtype, device=keys.device, max_query_len=min(MAX_QUERY_LEN, MAX_ROWS // group), **self._kw)
-        self.attention.bind_kv_contiguous(keys, values)
-        self.keys, self.values = keys, values
+        layer = PagedAttention(num_query_heads=self.num_query_heads, num_kv_heads=H, max_requests=B, token_capacity=cap,
+                               dtype=keys.dtype, device=keys.device, max_query_len=tokens, **self._kw)
+        layer.bind_kv_contiguous(keys, values)
+        return layer
 
     def build_cache(self, keys: torch.Tensor, values: torch.Tensor, queries: torch.Tensor | None = None) -> "EvictingCacheAdapter":
         """The prompt's keys and values (copied).  ``queries`` ``[batch, query_heads, W, 128]``: those of its last W
@@ -69,26 +68,29 @@ class EvictingCacheAdapter:
         k, v, self.positions, self.weights = buffers(max(S, room))
         k[:, :, :S], v[:, :, :S] = keys, values
         self.positions[:] = torch.arange(k.shape[2], dtype=torch.int32, device=dev)
-        self._layer(k, v)
+        self.attention, self.keys, self.values = self._layer(k, v), k, v
         self.lens = torch.full((B,), S, dtype=torch.int32, device=dev)
         self.query_pos = torch.full((B,), S - 1, dtype=torch.int32, device=dev)
         self.length = self.position = S
         self.evictions = 0
         if queries is not None:
-            W, step = queries.shape[2], self.attention.max_query_len
-            for lo in range(0, W, step):  # a few tokens at a time, each seeing what lies before it
+            # A few tokens at a time, each seeing what lies before it; a layer of their own, whose scores (8 tokens'
+            # against the one of a decode step) go with it.
+            W, step = queries.shape[2], min(MAX_QUERY_LEN, MAX_ROWS // (self.num_query_heads // H))
+            vote = self._layer(k, v, step)
+            for lo in range(0, W, step):
                 hi = min(lo + step, W)
                 at = torch.full_like(self.query_pos, S - W + hi - 1)
-                self.attention.forward(queries[:, :, lo:hi].transpose(1, 2), self.lens, key_pos=self.positions, query_pos=at,
-                                       mass=self.weights)
+                vote.forward(queries[:, :, lo:hi].transpose(1, 2), self.lens, key_pos=self.positions, query_pos=at, mass=self.weights)
+            del vote
         if S >= room:
             self._evict()
             if S > room:  # the long buffers are not needed any more
                 small = buffers(room)
                 for big, to in zip((self.keys, self.values, self.positions, self.weights), small):
                     to[:, :, : self.length] = big[:, :, : self.length]
-                self.positions, self.weights = small[2], small[3]
-                self._layer(small[0], small[1])
+                self.keys, self.values, self.positions, self.weights = small
+                self.attention = self._layer(self.keys, self.values)
         return self
 
     def _evict(self) -> None:

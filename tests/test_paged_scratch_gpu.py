@@ -58,3 +58,24 @@ def test_workspaces_are_sized_by_the_call():
         one = torch.zeros_like(m)
         att.forward(x, cache.seq_lens[:b], mass=one)
         assert torch.equal(one, m)
+
+
+@pytest.mark.parametrize("S", [2000, 8192], ids=["short", "past_the_budget"])
+def test_an_evicting_cache_keeps_the_scratch_of_one_token(S):
+    B, H, G, budget, interval = 8, 2, 4, 4096, 256
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda").to(BF)
+    keys, values, wq = r(B, H, S, D), r(B, H, S, D), r(B, H * G, 16, D)
+    ad = EvictingCacheAdapter(num_query_heads=H * G, num_kv_heads=H, budget=budget, interval=interval)
+    grown(ad.build_cache, keys, values, wq)
+    ad.decode_step(r(B, H * G, D), r(B, H, D), r(B, H, D))
+    room = budget + interval
+    rows = B * H * room
+    cache = 2 * rows * D * 2 + 8 * rows  # keys, values, positions, weights
+    one = rows * G * 4                    # the scores of a token
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    del ad
+    held = before - torch.cuda.memory_allocated()
+    evicting = 4 * B * H * (3 * budget + 8) if S > budget else 0
+    assert held < cache + one + evicting + 2 * MB, (held - cache) / one
