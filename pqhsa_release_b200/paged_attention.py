@@ -10,6 +10,8 @@ device: nothing here synchronises, and a captured call follows the lengths of it
 from __future__ import annotations
 
 import ctypes as C
+import threading
+import weakref
 from math import isfinite, sqrt
 
 import torch
@@ -22,6 +24,21 @@ _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cud
 _is_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
+class _Scratch:
+    """Scratch memory of one stream of execution; what launches recorded into a graph still use stays beside it."""
+
+    __slots__ = ("now", "kept", "__weakref__")
+
+    def __init__(self):
+        self.now, self.kept = None, []
+
+
+# (kind, device, thread, stream, capture) -> _Scratch, as long as a layer holds it.  Calls of one host thread on one stream
+# (or in one capture) run in order, whichever layer makes them; those of two threads can come between the two kernels
+# of an attention with weights.
+_SCRATCH: weakref.WeakValueDictionary = weakref.WeakValueDictionary()
+
+
 class PagedAttention:
     """The settings of one attention layer, a bound cache, and the workspaces its calls need.
 
@@ -30,9 +47,10 @@ class PagedAttention:
     first ``sink_tokens`` of its document; 0 = everything.  ``token_capacity``: most slots of a request, the last
     dimension of ``mass`` and ``key_pos``.
 
-    Calls on one stream run in order and share a workspace; every other stream, and every CUDA-graph capture, gets its
-    own (kept for the life of this object), so two streams or two graphs may run at once.  A graph replayed twice at
-    the same time shares its own.  One object is used by one host thread at a time."""
+    Calls of a host thread on one stream run in order and share a workspace, those of a model's other layers among
+    them; every other stream, and every CUDA-graph capture, gets its own (kept as long as a layer that used it), so two
+    streams or two graphs may run at once.  A graph replayed twice at the same time shares its own.  One object is used
+    by one host thread at a time."""
 
     def __init__(self, *, num_query_heads: int, num_kv_heads: int, max_requests: int, token_capacity: int, dtype: torch.dtype,
                  device: torch.device | str, max_query_len: int = 1, scale: float | None = None, softcap: float = 0.0,
@@ -79,8 +97,7 @@ class PagedAttention:
         self._sizes: dict = {}  # (requests, tokens) of a call -> workspace bytes without and with weights
         if 0 in self._workspace_bytes(self.max_requests, self.max_query_len):
             raise ValueError(_lib.lib.pqhsa_last_error_string().decode("utf-8", "replace"))
-        self._ws: dict = {}
-        self._kept: list = []
+        self._ws: dict = {}  # the shared scratch memory this layer has used
         self._kv_keepalive = None
         self._rows = 0  # requests the bound cache addresses
         self._forward_shape = self._append_shape = None  # shapes the blocks are set for (contiguous rows), or None
@@ -199,12 +216,15 @@ class PagedAttention:
         """(address, stream) of this stream's (or this capture's) scratch memory of that kind."""
         stream = _raw_stream(self._index)
         capturing = _is_capturing()
-        key = (kind, stream, _lib.lib.pqhsa_stream_capture_id(stream)) if capturing else (kind, stream)
-        t = self._ws.get(key)
+        key = (kind, self._index, threading.get_ident(), stream, _lib.lib.pqhsa_stream_capture_id(stream) if capturing else 0)
+        scratch = self._ws.get(key)
+        if scratch is None:
+            scratch = self._ws[key] = _SCRATCH.setdefault(key, _Scratch())
+        t = scratch.now
         if t is None or t.numel() < nbytes:
             if capturing and t is not None:
-                self._kept.append(t)  # launches recorded before still use it
-            t = self._ws[key] = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+                scratch.kept.append(t)  # launches recorded before still use it
+            t = scratch.now = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             if kind == "attention":
                 t[:4096].zero_()  # the kernels' counters
         return t.data_ptr(), stream

@@ -79,3 +79,76 @@ def test_an_evicting_cache_keeps_the_scratch_of_one_token(S):
     held = before - torch.cuda.memory_allocated()
     evicting = 4 * B * H * (3 * budget + 8) if S > budget else 0
     assert held < cache + one + evicting + 2 * MB, (held - cache) / one
+
+
+def test_the_layers_of_a_model_share_their_scratch():
+    """Sixteen layers of one step, eager and in captures of two sizes: what they hold beside the first layer's is nothing,
+    and each layer's results are its own."""
+    H, G, B, L = 2, 4, 6, 16
+    caches = [Cache([300, 77, 1, 0, 512, 130], H, BF, 16, "heads", seed=s) for s in range(L)]
+    qs = [queries(c, G, 1, s) for s, c in enumerate(caches)]
+    want = [ref.attend(c, q) for c, q in zip(caches, qs)]
+    outs = [torch.empty_like(q) for q in qs]
+    layers = [layer(c, G) for c in caches]
+
+    def steps(some, b=B):
+        for att, c, q, o in some:
+            att.forward(q[:b], c.seq_lens[:b], out=o[:b])
+
+    every = list(zip(layers, caches, qs, outs))
+    first, _ = grown(steps, every[:1])
+    assert first > 0 and grown(steps, every[1:])[0] == 0
+    for o, w in zip(outs, want):
+        check(o, None, w)
+    graphs = []
+    for b in (B, 2):
+        before = torch.cuda.memory_allocated()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            steps(every, b)
+        graphs.append((g, b, torch.cuda.memory_allocated() - before))
+    for g, b, held in graphs:
+        assert 0 < held <= first  # one workspace
+        for o in outs:
+            o.fill_(9.0)
+        g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            check(o[:b], None, tuple(x[:b] if torch.is_tensor(x) else x for x in w))
+    # a layer that is gone takes nothing along that the others use
+    del layers[0], every[0]
+    steps(every)
+    torch.cuda.synchronize()
+    for o, w in zip(outs[1:], want[1:]):
+        check(o, None, w)
+
+
+def test_two_threads_on_one_stream_do_not_share():
+    """An attention with weights is two kernels; another thread's call on the same stream can come between them."""
+    H, G = 2, 4
+    caches = [Cache([2000, 300], H, BF, 16, "heads", seed=s) for s in (1, 2)]
+    qs = [queries(c, G, 1, s) for s, c in enumerate(caches)]
+    layers = [layer(c, G) for c in caches]
+    masses = [torch.zeros(2, H, c.cap, device="cuda") for c in caches]
+    alone = []
+    for att, c, q in zip(layers, caches, qs):
+        m = torch.zeros(2, H, c.cap, device="cuda")
+        att.forward(q, c.seq_lens, mass=m)
+        alone.append(m)
+    torch.cuda.synchronize()
+
+    def work(i):
+        for _ in range(200):
+            layers[i].forward(qs[i], caches[i].seq_lens, mass=masses[i])
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for m, one in zip(masses, alone):
+        total = torch.zeros_like(m)
+        for _ in range(200):
+            total += one
+        assert torch.equal(m, total)
