@@ -18,6 +18,12 @@ from .decode_adapter import DecodeAttentionOutput, _squeeze_decode_token
 from .paged_attention import MAX_QUERY_LEN, MAX_ROWS, PagedAttention
 
 
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """Contiguous and on a 16-byte boundary, a copy if need be."""
+    x = x.contiguous()
+    return x.clone() if x.data_ptr() & 15 else x
+
+
 class EvictingCacheAdapter:
     """Up to ``budget + interval`` keys per (request, KV head); once that many are there, an eviction keeps ``budget``:
     the first ``sink_tokens`` and last ``recent`` positions and those of the largest accumulated weight.  ``softcap``,
@@ -114,10 +120,11 @@ class EvictingCacheAdapter:
         for x in (keys, values):  # before anything is counted or moved
             if x.dtype != self.keys.dtype or x.device != self.keys.device:
                 raise ValueError(f"keys and values must be {self.keys.dtype} tensors on {self.keys.device}, got {x.dtype} on {x.device}")
+        keys, values = _rows(keys), _rows(values)
         if self.length >= self.budget + self.interval:
             self._evict()
         self.query_pos.add_(1)
-        att.append(keys.contiguous(), values.contiguous(), self.lens, key_pos=self.positions, query_pos=self.query_pos, mass=self.weights)
+        att.append(keys, values, self.lens, key_pos=self.positions, query_pos=self.query_pos, mass=self.weights)
         self.length += 1
         self.position += 1
 

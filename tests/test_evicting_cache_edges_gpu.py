@@ -1,0 +1,50 @@
+"""Calls of the evicting adapter at its edges: odd inputs, refusals that must change nothing, captures."""
+
+import pytest
+import torch
+
+from paged_ref import D
+from pqhsa_release_b200 import EvictingCacheAdapter
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def rows(*shape, dtype=BF, seed=0):
+    return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dtype)
+
+
+def state(ad):
+    """Everything an adapter is, its device tensors copied."""
+    return ((ad.length, ad.position, ad.evictions, id(ad.attention)),
+            [t.clone() for t in (ad.keys, ad.values, ad.positions, ad.weights, ad.lens, ad.query_pos)])
+
+
+def same(a, b):
+    return a[0] == b[0] and all(torch.equal(x, y) for x, y in zip(a[1], b[1]))
+
+
+def filled(dtype=BF, tokens=40, **kw):
+    """An adapter of two requests whose next append evicts."""
+    ad = EvictingCacheAdapter(num_query_heads=8, num_kv_heads=2, budget=32, interval=8, sink_tokens=2, recent=4, **kw)
+    k, v = rows(2, 2, tokens, D, dtype=dtype, seed=1), rows(2, 2, tokens, D, dtype=dtype, seed=2)
+    ad.build_cache(k[:, :, : tokens - 1], v[:, :, : tokens - 1])
+    ad.append(k[:, :, tokens - 1], v[:, :, tokens - 1])
+    return ad
+
+
+def shifted(x):
+    """The same values one element off a 16-byte boundary, contiguous."""
+    odd = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape)
+    return odd.copy_(x)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+def test_rows_off_a_16_byte_boundary(dtype):
+    a, b = filled(dtype), filled(dtype)
+    for i in range(12):
+        k, v, q = rows(2, 2, D, dtype=dtype, seed=10 + i), rows(2, 2, D, dtype=dtype, seed=30 + i), rows(2, 8, D, dtype=dtype, seed=50 + i)
+        want = a.decode_step(q, k, v).context
+        assert torch.equal(b.decode_step(q, shifted(k), shifted(v) if i % 2 else v).context, want), i
+    sa, sb = state(a), state(b)
+    assert sa[0][:3] == sb[0][:3] == (36, 52, 2) and all(torch.equal(x, y) for x, y in zip(sa[1], sb[1]))
