@@ -128,18 +128,29 @@ class EvictingCacheAdapter:
         self.length += 1
         self.position += 1
 
+    def _queries(self, queries: torch.Tensor) -> torch.Tensor:
+        """Checked, and as rows that the attention can read."""
+        if queries.ndim != 3 or queries.shape != (self.keys.shape[0], self.num_query_heads, _lib.HEAD_DIM):
+            raise ValueError(f"queries must be [{self.keys.shape[0]}, {self.num_query_heads}, 128]")
+        if queries.dtype != self.keys.dtype or queries.device != self.keys.device:
+            raise ValueError(f"queries must be a {self.keys.dtype} tensor on {self.keys.device}, got {queries.dtype} on {queries.device}")
+        fit = 16 // queries.element_size()  # strided rows are read in place where they lie on 16-byte boundaries
+        if queries.stride(2) == 1 and not (queries.stride(0) % fit or queries.stride(1) % fit or queries.data_ptr() & 15):
+            return queries
+        return _rows(queries)
+
     def forward(self, queries: torch.Tensor) -> DecodeAttentionOutput:
         """The last token's attention; its weights are accumulated."""
         att = self._ready()
-        if queries.ndim != 3 or queries.shape != (self.keys.shape[0], self.num_query_heads, _lib.HEAD_DIM):
-            raise ValueError(f"queries must be [{self.keys.shape[0]}, {self.num_query_heads}, 128]")
-        return DecodeAttentionOutput(context=att.forward(queries, self.lens, key_pos=self.positions, query_pos=self.query_pos,
-                                                         mass=self.weights))
+        return DecodeAttentionOutput(context=att.forward(self._queries(queries), self.lens, key_pos=self.positions,
+                                                         query_pos=self.query_pos, mass=self.weights))
 
     def decode_step(self, queries: torch.Tensor, keys: torch.Tensor | None = None, values: torch.Tensor | None = None, *,
                     append_kv: bool = True) -> DecodeAttentionOutput:
         if append_kv:
             if keys is None or values is None:
                 raise ValueError("keys and values are required when append_kv=True")
+            self._ready()
+            queries = self._queries(queries)  # a refused step appends nothing
             self.append(keys, values)
         return self.forward(queries)

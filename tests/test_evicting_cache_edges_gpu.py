@@ -48,3 +48,29 @@ def test_rows_off_a_16_byte_boundary(dtype):
         assert torch.equal(b.decode_step(q, shifted(k), shifted(v) if i % 2 else v).context, want), i
     sa, sb = state(a), state(b)
     assert sa[0][:3] == sb[0][:3] == (36, 52, 2) and all(torch.equal(x, y) for x, y in zip(sa[1], sb[1]))
+
+
+def test_a_step_with_bad_queries_appends_nothing():
+    ad = filled()
+    before = state(ad)
+    k, v, q = rows(2, 2, D, seed=3), rows(2, 2, D, seed=4), rows(2, 8, D, seed=5)
+    for bad in (q[:1], q[:, :4], q[:, :, :64], q.float(), q.cpu(), q[0], q.to(HF)):
+        with pytest.raises(ValueError, match="queries"):
+            ad.decode_step(bad, k, v)
+        assert same(state(ad), before), tuple(bad.shape)
+    assert ad.decode_step(q, k, v).context.shape == q.shape and ad.position == 41
+    with pytest.raises(RuntimeError, match="build_cache"):
+        EvictingCacheAdapter(num_query_heads=8, num_kv_heads=2, budget=32, recent=4).decode_step(q, k, v)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32], ids=["bf16", "fp16", "fp32"])
+def test_queries_in_any_strides(dtype):
+    ad = filled(dtype)
+    q = rows(2, 8, D, dtype=dtype, seed=5)
+    want = ad.forward(q).context
+    wide = torch.empty(2, 9, 2 * D, dtype=dtype, device="cuda")
+    forms = [wide[:, 1:, :D], wide[:, :8, 4 : 4 + D], wide[:, :8, ::2], torch.empty(8, 2, D, dtype=dtype, device="cuda").transpose(0, 1),
+             torch.empty(2, D, 8, dtype=dtype, device="cuda").transpose(1, 2), torch.empty(2 * 8 * D + 1, dtype=dtype, device="cuda")[1:].view(2, 8, D)]
+    for f in forms:
+        f.copy_(q)
+        assert torch.equal(ad.forward(f).context, want), f.stride()
