@@ -19,9 +19,11 @@ from .paged_attention import MAX_QUERY_LEN, MAX_ROWS, PagedAttention
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    """Contiguous and on a 16-byte boundary, a copy if need be."""
-    x = x.contiguous()
-    return x.clone() if x.data_ptr() & 15 else x
+    """Rows that the kernels can read: as they are where they lie in one piece on 16-byte boundaries, else a copy."""
+    fit = 16 // x.element_size()
+    if x.stride(-1) == 1 and not (x.data_ptr() & 15 or any(s % fit for s in x.stride()[:-1])):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 class EvictingCacheAdapter:
@@ -71,32 +73,37 @@ class EvictingCacheAdapter:
             k, v = (torch.zeros(B, H, cap, D, dtype=keys.dtype, device=dev) for _ in range(2))
             return k, v, torch.zeros(B, H, cap, dtype=torch.int32, device=dev), torch.zeros(B, H, cap, device=dev)
 
-        k, v, self.positions, self.weights = buffers(max(S, room))
+        # the adapter takes all of it over at the end: a prompt that is refused leaves the cache there was
+        k, v, positions, weights = buffers(max(S, room))
         k[:, :, :S], v[:, :, :S] = keys, values
-        self.positions[:] = torch.arange(k.shape[2], dtype=torch.int32, device=dev)
-        self.attention, self.keys, self.values = self._layer(k, v), k, v
-        self.lens = torch.full((B,), S, dtype=torch.int32, device=dev)
-        self.query_pos = torch.full((B,), S - 1, dtype=torch.int32, device=dev)
-        self.length = self.position = S
-        self.evictions = 0
+        positions[:] = torch.arange(k.shape[2], dtype=torch.int32, device=dev)
+        layer = self._layer(k, v)
+        lens = torch.full((B,), S, dtype=torch.int32, device=dev)
+        query_pos = torch.full((B,), S - 1, dtype=torch.int32, device=dev)
+        length, evictions = S, 0
         if queries is not None:
             # A few tokens at a time, each seeing what lies before it; a layer of their own, whose scores (8 tokens'
             # against the one of a decode step) go with it.
+            queries = _rows(queries)
             W, step = queries.shape[2], min(MAX_QUERY_LEN, MAX_ROWS // (self.num_query_heads // H))
             vote = self._layer(k, v, step)
             for lo in range(0, W, step):
                 hi = min(lo + step, W)
-                at = torch.full_like(self.query_pos, S - W + hi - 1)
-                vote.forward(queries[:, :, lo:hi].transpose(1, 2), self.lens, key_pos=self.positions, query_pos=at, mass=self.weights)
+                at = torch.full_like(query_pos, S - W + hi - 1)
+                vote.forward(queries[:, :, lo:hi].transpose(1, 2), lens, key_pos=positions, query_pos=at, mass=weights)
             del vote
         if S >= room:
-            self._evict()
+            layer.evict(lens, mass=weights, key_pos=positions, query_pos=query_pos, budget=self.budget, recent=self.recent)
+            length, evictions = self.budget, 1
             if S > room:  # the long buffers are not needed any more
                 small = buffers(room)
-                for big, to in zip((self.keys, self.values, self.positions, self.weights), small):
-                    to[:, :, : self.length] = big[:, :, : self.length]
-                self.keys, self.values, self.positions, self.weights = small
-                self.attention = self._layer(self.keys, self.values)
+                for big, to in zip((k, v, positions, weights), small):
+                    to[:, :, :length] = big[:, :, :length]
+                k, v, positions, weights = small
+                layer = self._layer(k, v)
+        self.attention, self.keys, self.values, self.positions, self.weights = layer, k, v, positions, weights
+        self.lens, self.query_pos = lens, query_pos
+        self.length, self.position, self.evictions = length, S, evictions
         return self
 
     def _evict(self) -> None:
@@ -120,7 +127,7 @@ class EvictingCacheAdapter:
         for x in (keys, values):  # before anything is counted or moved
             if x.dtype != self.keys.dtype or x.device != self.keys.device:
                 raise ValueError(f"keys and values must be {self.keys.dtype} tensors on {self.keys.device}, got {x.dtype} on {x.device}")
-        keys, values = _rows(keys), _rows(values)
+        keys, values = _rows(keys.contiguous()), _rows(values.contiguous())
         if self.length >= self.budget + self.interval:
             self._evict()
         self.query_pos.add_(1)
@@ -134,9 +141,6 @@ class EvictingCacheAdapter:
             raise ValueError(f"queries must be [{self.keys.shape[0]}, {self.num_query_heads}, 128]")
         if queries.dtype != self.keys.dtype or queries.device != self.keys.device:
             raise ValueError(f"queries must be a {self.keys.dtype} tensor on {self.keys.device}, got {queries.dtype} on {queries.device}")
-        fit = 16 // queries.element_size()  # strided rows are read in place where they lie on 16-byte boundaries
-        if queries.stride(2) == 1 and not (queries.stride(0) % fit or queries.stride(1) % fit or queries.data_ptr() & 15):
-            return queries
         return _rows(queries)
 
     def forward(self, queries: torch.Tensor) -> DecodeAttentionOutput:

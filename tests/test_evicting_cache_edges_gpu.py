@@ -74,3 +74,46 @@ def test_queries_in_any_strides(dtype):
     for f in forms:
         f.copy_(q)
         assert torch.equal(ad.forward(f).context, want), f.stride()
+
+
+@pytest.mark.parametrize("why", ["queries_elsewhere", "values_shape", "queries_dtype", "group", "dtype"])
+def test_a_refused_prompt_leaves_the_cache_there_was(why):
+    ad = filled()
+    before = state(ad)
+    k, wq = rows(2, 2, 60, D, seed=8), rows(2, 8, 5, D, seed=9)
+    values, queries = k, wq
+    if why == "queries_elsewhere":
+        queries = wq.cpu()
+    elif why == "values_shape":
+        values = k[:, :, :-1]
+    elif why == "queries_dtype":
+        queries = wq.float()
+    elif why == "dtype":
+        k = values = k.double()
+        queries = wq.double()
+    if why == "group":  # 32 query heads per KV head: more than a layer takes
+        ad = EvictingCacheAdapter(num_query_heads=64, num_kv_heads=2, budget=32, interval=8, recent=4)
+        with pytest.raises(ValueError, match="query heads per KV head"):
+            ad.build_cache(k, values)
+        with pytest.raises(RuntimeError, match="build_cache"):
+            ad.append(k[:, :, 0], k[:, :, 0])
+        return
+    with pytest.raises(ValueError):
+        ad.build_cache(k, values, queries)
+    assert same(state(ad), before)
+    q = rows(2, 8, D, seed=5)
+    twin = filled()
+    twin.append(rows(2, 2, D, seed=3), rows(2, 2, D, seed=4))
+    ad.append(rows(2, 2, D, seed=3), rows(2, 2, D, seed=4))
+    assert torch.equal(ad.forward(q).context, twin.forward(q).context)
+
+
+def test_a_prompts_queries_in_any_strides():
+    k, v, wq = rows(2, 2, 60, D, seed=8), rows(2, 2, 60, D, seed=6), rows(2, 8, 13, D, seed=9)
+    a = EvictingCacheAdapter(num_query_heads=8, num_kv_heads=2, budget=32, interval=8, sink_tokens=2, recent=4).build_cache(k, v, wq)
+    odd = shifted(wq)
+    wide = torch.empty(2, 13, 8, D + 4, dtype=BF, device="cuda")[..., 4:].transpose(1, 2)
+    wide.copy_(wq)
+    for q in (odd, wide, wq.transpose(1, 2).contiguous().transpose(1, 2)):
+        b = EvictingCacheAdapter(num_query_heads=8, num_kv_heads=2, budget=32, interval=8, sink_tokens=2, recent=4).build_cache(k, v, q)
+        assert all(torch.equal(x, y) for x, y in zip(state(a)[1], state(b)[1]))
