@@ -29,7 +29,10 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 class EvictingCacheAdapter:
     """Up to ``budget + interval`` keys per (request, KV head); once that many are there, an eviction keeps ``budget``:
     the first ``sink_tokens`` and last ``recent`` positions and those of the largest accumulated weight.  ``softcap``,
-    ``alibi_slopes`` and ``window`` as for :class:`PagedAttention`."""
+    ``alibi_slopes`` and ``window`` as for :class:`PagedAttention`.
+
+    Which step evicts is counted on the host, so ``build_cache`` and ``append`` refuse to be captured into a CUDA graph
+    (``RuntimeError``); ``forward`` can be, and so can a loop of :class:`PagedAttention`'s own calls."""
 
     def __init__(self, *, num_query_heads: int, num_kv_heads: int, budget: int, interval: int = 256, sink_tokens: int = 4,
                  recent: int = 128, scale: float | None = None, softcap: float = 0.0,
@@ -47,6 +50,11 @@ class EvictingCacheAdapter:
         self.evictions = 0
 
     # ---- cache -------------------------------------------------------------------------------------------
+    @staticmethod
+    def _not_captured(call: str) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{call} counts on the host when to evict and cannot be captured into a CUDA graph")
+
     def _layer(self, keys: torch.Tensor, values: torch.Tensor, tokens: int = 1) -> PagedAttention:
         """A layer over these contiguous buffers; positions and weights are [batch, kv_heads, capacity] as they."""
         B, H, cap, _ = keys.shape
@@ -67,6 +75,8 @@ class EvictingCacheAdapter:
         if queries is not None and (queries.ndim != 4 or queries.shape[:2] != (B, self.num_query_heads) or queries.shape[3] != D
                                     or not 1 <= queries.shape[2] <= S or queries.dtype != keys.dtype):
             raise ValueError(f"queries must be [{B}, {self.num_query_heads}, 1..{S}, 128] in the keys' dtype")
+        if keys.is_cuda:
+            self._not_captured("build_cache")
         dev, room = keys.device, self.budget + self.interval
 
         def buffers(cap):
@@ -127,6 +137,7 @@ class EvictingCacheAdapter:
         for x in (keys, values):  # before anything is counted or moved
             if x.dtype != self.keys.dtype or x.device != self.keys.device:
                 raise ValueError(f"keys and values must be {self.keys.dtype} tensors on {self.keys.device}, got {x.dtype} on {x.device}")
+        self._not_captured("append")
         keys, values = _rows(keys.contiguous()), _rows(values.contiguous())
         if self.length >= self.budget + self.interval:
             self._evict()

@@ -117,3 +117,38 @@ def test_a_prompts_queries_in_any_strides():
     for q in (odd, wide, wq.transpose(1, 2).contiguous().transpose(1, 2)):
         b = EvictingCacheAdapter(num_query_heads=8, num_kv_heads=2, budget=32, interval=8, sink_tokens=2, recent=4).build_cache(k, v, q)
         assert all(torch.equal(x, y) for x, y in zip(state(a)[1], state(b)[1]))
+
+
+def test_what_counts_on_the_host_is_not_captured():
+    """Replays of a captured append would go past the room without an eviction, and their rows would be dropped."""
+    ad = filled()
+    ad.append(rows(2, 2, D, seed=3), rows(2, 2, D, seed=4))
+    before = state(ad)
+    k, v, q = rows(2, 2, D, seed=13), rows(2, 2, D, seed=14), rows(2, 8, D, seed=5)
+    calls = {"append": lambda: ad.append(k, v), "decode": lambda: ad.decode_step(q, k, v), "build": lambda: ad.build_cache(k[:, :, None], v[:, :, None])}
+    for name, call in calls.items():
+        one, g = torch.zeros(1, device="cuda"), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            one.add_(1.0)  # the capture itself goes on
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+        g.replay()
+        torch.cuda.synchronize()
+        assert one.item() == 1.0 and same(state(ad), before), name
+    # the attention alone: each replay accumulates its weights, as an eager call does
+    twin = filled()
+    twin.append(rows(2, 2, D, seed=3), rows(2, 2, D, seed=4))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ad.forward(q).context
+    for _ in range(3):
+        g.replay()
+        want = twin.forward(q).context
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(ad.weights, twin.weights)
+    ad.append(k, v)
+    twin.append(k, v)
+    g.replay()
+    want = twin.forward(q).context
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(ad.weights, twin.weights)
