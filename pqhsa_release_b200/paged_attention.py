@@ -43,7 +43,7 @@ class PagedAttention:
     """The settings of one attention layer, a bound cache, and the workspaces its calls need.
 
     ``softcap``: scores become ``softcap * tanh(score / softcap)``.  ``alibi_slopes`` ``[num_query_heads]``: minus slope
-    times distance.  ``window`` / ``sink_tokens``: a token sees the last ``window`` positions (itself included) and the
+    times distance (copied).  ``window`` / ``sink_tokens``: a token sees the last ``window`` positions (itself included) and the
     first ``sink_tokens`` of its document; 0 = everything.  ``token_capacity``: most slots of a request, the last
     dimension of ``mass`` and ``key_pos``.
 
@@ -84,7 +84,7 @@ class PagedAttention:
         if alibi_slopes is not None:
             if tuple(alibi_slopes.shape) != (self.Hq,):
                 raise ValueError(f"alibi_slopes must have one entry per query head, got {tuple(alibi_slopes.shape)}")
-            self.alibi_slopes = alibi_slopes.detach().to(device=self.device, dtype=torch.float32).contiguous().clone()
+            self.alibi_slopes = self._slopes(alibi_slopes.detach())
         # one argument block per operator (each keeps the sizes of its last call), the cache's part the same in all
         self.p, self._append_p, self._evict_p = _lib.PagedParams(), _lib.PagedParams(), _lib.PagedParams()
         for p in (self.p, self._append_p, self._evict_p):
@@ -152,6 +152,18 @@ class PagedAttention:
             p.stride_block, p.stride_head, p.stride_row = strides
             p.block_table, p.max_blocks = table, max_blocks
         self._forward_shape = self._append_shape = None
+
+    def _slopes(self, given: torch.Tensor) -> torch.Tensor:
+        """A copy that every stream may read.  During a capture a copy would only be there once the graph has run: then the
+        tensor itself."""
+        slopes = given.to(device=self.device, dtype=torch.float32).contiguous()
+        with torch.cuda.device(self._index):
+            if not _is_capturing():
+                slopes = slopes.clone()
+                torch.cuda.current_stream().synchronize()
+            elif slopes.data_ptr() != given.data_ptr():
+                raise RuntimeError(f"a layer made during a CUDA-graph capture needs its alibi_slopes as a contiguous float32 tensor on {self.device}")
+        return slopes
 
     # ---- checks and scratch ------------------------------------------------------------------------------
     def _check(self, t: torch.Tensor, name: str, dtype: torch.dtype) -> None:
