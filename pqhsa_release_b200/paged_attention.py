@@ -281,6 +281,8 @@ class PagedAttention:
             p.requests, p.query_len = self._tokens(shape, "q", self.Hq)
             self._bytes = self._workspace_bytes(p.requests, p.query_len)
             p.q_stride_request, p.q_stride_token, p.q_stride_head = self._strides_of(q, "q")
+            if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+                raise ValueError("rows of out must not lie on one another")
             p.out_stride_request, p.out_stride_token, p.out_stride_head = self._strides_of(out, "out")
             self._forward_shape = shape if even else None
         B = shape[0]
