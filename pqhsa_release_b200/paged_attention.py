@@ -68,8 +68,9 @@ class PagedAttention:
         if max_requests < 1 or token_capacity < 1:
             raise ValueError("max_requests and token_capacity must be positive")
         scale = 1.0 / sqrt(_lib.HEAD_DIM) if scale is None else float(scale)
-        if not isfinite(scale) or not isfinite(softcap) or softcap < 0:
-            raise ValueError("scale must be finite and softcap finite and non-negative")
+        kept = [C.c_float(x).value for x in (scale, softcap)]  # as the kernels get them
+        if not all(map(isfinite, kept)) or softcap < 0 or (kept[1] == 0.0) != (softcap == 0.0):
+            raise ValueError("scale must be finite and softcap finite and non-negative, in 32 bits too")
         if window < 0 or sink_tokens < 0:
             raise ValueError("window and sink_tokens must be non-negative")
         self.device = torch.device(device)
