@@ -12,7 +12,8 @@ namespace pqhsa {
 constexpr int kPagedGroupRows = 32;    // query rows of one KV head that go through the cache together
 constexpr int kPagedMaxRows = 64;      // query_len * group at most: two passes of kPagedGroupRows
 constexpr int kPagedMaxQuery = 8;
-constexpr int kPagedMaxCtas = 1024;    // counters in the workspace (one per CTA of the attention kernel)
+constexpr int kPagedMassCtas = 4;      // CTAs of the weights' kernel on an SM (the attention has one)
+constexpr int kPagedMaxCtas = 1024;    // counters in the workspace, one per CTA of a kernel, of which there are fewer than this
 
 struct PagedArgs {
   const void* k_base;
@@ -266,7 +267,7 @@ __device__ __forceinline__ bool paged_locate(const PagedArgs& a, int ctas, int c
   if (aligned) {
     sh.c0 = cta - i;
     sh.parts = unit;
-    sh.x = c.tile = c.g.tiles * i / unit;  // fits 31 bits: at most 2^21 tiles and 2^10 CTAs
+    sh.x = c.tile = c.g.tiles * i / unit;  // fits 31 bits: at most 2^21 tiles and 2^10 - 1 CTAs (the host sees to both)
     sh.x_end = c.g.tiles * (i + 1) / unit;
   } else {
     c.tile = i;

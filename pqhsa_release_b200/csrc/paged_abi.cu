@@ -120,7 +120,8 @@ int pqhsa_paged_attention(const pqhsa_paged_params* p, void* stream) {
     return set_error(PQHSA_E_SHAPE, "scale must be finite, softcap finite, non-negative and not vanishing against scale");
   if (!p->workspace || ((uintptr_t)p->workspace & 255))
     return set_error(PQHSA_E_WORKSPACE, "workspace missing or not 256-byte aligned");
-  if (sm_count() > kPagedMaxCtas) return set_error(PQHSA_E_CAPACITY, "more than %d SMs", kPagedMaxCtas);
+  if (sm_count() * kPagedMassCtas >= kPagedMaxCtas)
+    return set_error(PQHSA_E_CAPACITY, "more than %d SMs", (kPagedMaxCtas - 1) / kPagedMassCtas);
   const PagedWs w = paged_ws(p);
   if (p->workspace_bytes < w.total)
     return set_error(PQHSA_E_WORKSPACE, "workspace has %zu bytes, %zu needed", p->workspace_bytes, w.total);

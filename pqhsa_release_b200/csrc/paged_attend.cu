@@ -998,7 +998,7 @@ __global__ void __launch_bounds__(kMassThreads) paged_mass_kernel(const PagedArg
 int launch_paged_mass(const PagedArgs& a, cudaStream_t st) {
   PagedArgs b = a;
   b.groups = 1;
-  if (paged_launch(paged_mass_kernel, dim3(sm_count() * 4), kMassThreads, 0, st, 0, b) != cudaSuccess) return check_launch("paged_mass");
+  if (paged_launch(paged_mass_kernel, dim3(sm_count() * kPagedMassCtas), kMassThreads, 0, st, 0, b) != cudaSuccess) return check_launch("paged_mass");
   return PQHSA_OK;
 }
 
