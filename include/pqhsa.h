@@ -423,7 +423,12 @@ int pqhsa_topk_radix(const float* scores, int32_t rows, int32_t n, int64_t row_s
  * the output sum e^s v / sum e^s, lse = ln sum e^s, and with mass  mass[r, h, i] += sum over tokens and the group's
  * heads of e^s / sum e^s.  A token that sees no key has output 0 and lse -inf.  Keys that no token sees are not read:
  * their slots may hold anything.  A block-table entry outside 0 .. num_blocks - 1 means "not in the cache": its keys
- * are invisible.  n is clamped to 0 .. min(slot_capacity, max_blocks * block_size); n <= 0 is an idle request. */
+ * are invisible.  n is clamped to 0 .. min(slot_capacity, max_blocks * block_size); n <= 0 is an idle request.
+ *
+ * Scores, sums, lse and mass are fp32 whatever the types.  With a 16-bit cache the weights e^s are rounded to its type for
+ * the product with V, and the sum they are divided by is not: beside its own rounding an output is off by at most half a
+ * step of that type (bf16 2^-8, fp16 2^-11) of sum e^s |v| / sum e^s; fp16 weights below 2^-27 of the row's largest by
+ * at most 2^-38 of it each. */
 typedef struct pqhsa_paged_params {
   int32_t abi_version;     /* PQHSA_ABI_VERSION */
   int32_t dtype;           /* enum pqhsa_dtype of q, K/V and out */

@@ -478,7 +478,9 @@ static int launch_fp32(const PagedArgs& a, cudaStream_t st) {
 // layout with one 8x8 transpose in registers per 8 keys.  A thread holds the same two query rows of every 8 in S^T and
 // in O^T, so maxima, sums and rescaling need no exchange.  p is rounded to the 16-bit type for the product with V (half
 // a step; the sum it is divided by adds them unrounded in 32 bits).  Against one row per m16 (P V with 16 rows
-// of which 4 or 8 are real) this halves the instructions and the accumulators.
+// of which 4 or 8 are real) this halves the instructions and the accumulators.  A second product with what the rounding
+// took off p brings the error against 64 bits from 2.4e-3 to the output's own 1.7e-3 (bf16), but costs 1-2 % up to 8
+// rows, 8 % for 16 and 20-30 % for more, and makes a NaN of an infinite value whose p is rounded to itself: not taken.
 //
 // fp16 has no numbers between 0 and 2^-24, and few bits below 2^-14: with p = 2^(s - m) at most 2^8, thousands of keys some
 // 17 nats below one loud key (a sink) would vanish from the product while the sum counts them.  Its p are therefore
@@ -1002,10 +1004,18 @@ int launch_paged_mass(const PagedArgs& a, cudaStream_t st) {
   return PQHSA_OK;
 }
 
+// Accumulators of the 8, 16 or 32 rows nearest above those there are (of more than 32, 32 to a pass).  With 32 rows the merge
+// buffer leaves room for a ring of two tiles a warp instead of three, and 10 registers a thread are spilled (29 with a cap or bias).  us over
+// 4 x 128K keys of 8 KV heads in bf16, 328 at the copy rate: 8 rows 312, 16 rows 330, 24 rows 370, 32 rows 386 (capped
+// 480); 40 to 64 rows, whose two passes both read the keys, 693.
 template <typename E, bool SHAPED> static int launch_16bit(const PagedArgs& a, int rows, cudaStream_t st) {
   return rows <= 8 ? launch_mma<E, 1, 3, SHAPED>(a, st) : rows <= 16 ? launch_mma<E, 2, 3, SHAPED>(a, st) : launch_mma<E, 4, 2, SHAPED>(a, st);
 }
 
+// fp32: few rows wait for memory, and twelve warps with two tiles each ask for more of it than eight with three; from 16
+// rows on the products are what takes the time, and the accumulators leave registers for eight warps.  us over 4 x 32K keys
+// (164 at the copy rate), 12 x 2 | 8 x 3 | 8 x 2: 4 rows 161 | 209 | 195, 8 rows 235 | 286 | 285, 16 rows 454 | 443 | 440,
+// 32 rows - | 1042 | 1038, 64 rows (two passes) 2058.  One request of 1K: 4 rows 9.1 | 8.6 | 8.4.
 int launch_paged_attend(const PagedArgs& a, int dtype, cudaStream_t st) {
   PagedArgs b = a;
   const int rows = a.R < kPagedGroupRows ? a.R : kPagedGroupRows;

@@ -17,7 +17,7 @@
 // that is summed through distributed shared memory, then number the holes and the kept slots behind the budget in slot order
 // and write both lists.  The moves go over the whole GPU, four to a warp, all their loads in flight before the stores:
 // they are the bytes of the operator (4 rows a move against 8 bytes a slot for the selection).  One B200, 32 streams from
-// 131072 slots down to 16384: selection 28 us (34 MB read; three passes with a cluster barrier each), moves 90 us
+// 131072 slots down to 16384: selection 29 us (34 MB read; three passes with a cluster barrier each), moves 90 us
 // (470 MB, 5.2 TB/s with rows of 256 bytes in random order; eight to a warp and four CTAs to an SM 4 us more).
 #include <cooperative_groups.h>
 
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(256, kEvMoveCtas<E>) evict_move_kernel(const P
 int launch_paged_evict(const PagedArgs& a, const PagedEvict& e, int dtype, cudaStream_t st) {
   // CTAs per stream: enough that a share fits shared memory twice over, and with few streams enough to use the GPU.
   // The histograms of a cluster cross its network: on 32 streams of 128K slots 8 CTAs of 512 threads took 47 us where
-  // 4 of 1024 took 33, now 28 (2 CTAs of an SM ask for 128 KB a pass); on 8 streams of 4352 slots one CTA takes 13 us, two 15.
+  // 4 of 1024 took 33, now 29 (2 CTAs of an SM ask for 128 KB a pass); on 8 streams of 4352 slots one CTA takes 13 us, two 15.
   int ranks = 1;
   while (ranks < 8 && (a.limit > ranks * 32768 || (a.limit > ranks * 8192 && a.B * a.H * ranks * 2 <= sm_count()))) ranks *= 2;
   const int share = ((a.limit + ranks - 1) / ranks + 127) / 128 * 128;

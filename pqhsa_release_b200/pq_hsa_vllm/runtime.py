@@ -331,7 +331,8 @@ def run_pq_decode_mq(impl, layer, query, key, value, kv_cache, attn_metadata, ou
 
 def dense_enabled() -> bool:
     """PQ_HSA_DENSE=1 (default 0): decode steps that the PQ path does not take - contexts too short for an index, a batch
-    with such a request, requests without ids - run on this library's dense kernel instead of the original forward."""
+    with such a request, requests without ids, all of them with PQ_HSA_ENABLE=0 - run on this library's dense kernel
+    instead of the original forward."""
     return os.environ.get("PQ_HSA_DENSE", "0") == "1"
 
 
