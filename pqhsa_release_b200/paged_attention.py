@@ -25,17 +25,27 @@ _is_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 class _Scratch:
-    """Scratch memory of one stream of execution; what launches recorded into a graph still use stays beside it."""
+    """Scratch memory of one stream of execution.  Whoever uses it holds ``lock`` from ``take`` until the call's launches
+    are made: those of another thread may not come between them."""
 
-    __slots__ = ("now", "kept", "__weakref__")
+    __slots__ = ("now", "kept", "lock", "__weakref__")
 
     def __init__(self):
-        self.now, self.kept = None, []
+        self.now, self.kept, self.lock = None, [], threading.Lock()
+
+    def take(self, nbytes: int, device: torch.device, counters: bool, capturing: bool) -> int:
+        t = self.now
+        if t is None or t.numel() < nbytes:
+            if capturing and t is not None:
+                self.kept.append(t)  # launches recorded before still use it
+            t = self.now = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            if counters:
+                t[:4096].zero_()
+        return t.data_ptr()
 
 
-# (kind, device, thread, stream, capture) -> _Scratch, as long as a layer holds it.  Calls of one host thread on one stream
-# (or in one capture) run in order, whichever layer makes them; those of two threads can come between the two kernels
-# of an attention with weights.
+# (kind, device, stream, capture) -> _Scratch, as long as a layer holds it: the calls made on one stream, or recorded into
+# one capture, run in order, whichever layer makes them.
 _SCRATCH: weakref.WeakValueDictionary = weakref.WeakValueDictionary()
 
 
@@ -47,10 +57,10 @@ class PagedAttention:
     first ``sink_tokens`` of its document; 0 = everything.  ``token_capacity``: most slots of a request, the last
     dimension of ``mass`` and ``key_pos``.
 
-    Calls of a host thread on one stream run in order and share a workspace, those of a model's other layers among
-    them; every other stream, and every CUDA-graph capture, gets its own (kept as long as a layer that used it), so two
-    streams or two graphs may run at once.  A graph replayed twice at the same time shares its own.  One object is used
-    by one host thread at a time."""
+    Calls on one stream run in order and share a workspace, those of a model's other layers among them; every other
+    stream, and every CUDA-graph capture, gets its own (kept as long as a layer that used it), so two streams or two
+    graphs may run at once.  A graph replayed twice at the same time shares its own.  One object is used by one host
+    thread at a time."""
 
     def __init__(self, *, num_query_heads: int, num_kv_heads: int, max_requests: int, token_capacity: int, dtype: torch.dtype,
                  device: torch.device | str, max_query_len: int = 1, scale: float | None = None, softcap: float = 0.0,
@@ -225,22 +235,15 @@ class PagedAttention:
             got = self._sizes[requests, tokens] = tuple(got)
         return got
 
-    def _scratch(self, kind: str, nbytes: int) -> tuple[int, int]:
-        """(address, stream) of this stream's (or this capture's) scratch memory of that kind."""
+    def _scratch(self, kind: str) -> tuple[_Scratch, int, bool]:
+        """The scratch memory of that kind of this stream (or this capture), the stream, and whether it is being captured."""
         stream = _raw_stream(self._index)
         capturing = _is_capturing()
-        key = (kind, self._index, threading.get_ident(), stream, _lib.lib.pqhsa_stream_capture_id(stream) if capturing else 0)
+        key = (kind, self._index, stream, _lib.lib.pqhsa_stream_capture_id(stream) if capturing else 0)
         scratch = self._ws.get(key)
         if scratch is None:
             scratch = self._ws[key] = _SCRATCH.setdefault(key, _Scratch())
-        t = scratch.now
-        if t is None or t.numel() < nbytes:
-            if capturing and t is not None:
-                scratch.kept.append(t)  # launches recorded before still use it
-            t = scratch.now = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
-            if kind == "attention":
-                t[:4096].zero_()  # the kernels' counters
-        return t.data_ptr(), stream
+        return scratch, stream, capturing
 
     def _positions(self, p, B: int, key_pos, query_pos, mass) -> None:
         p.key_pos = None if key_pos is None else self._per_slot(key_pos, "key_pos", torch.int32, B)
@@ -299,8 +302,10 @@ class PagedAttention:
             raise ValueError("key_pos needs query_pos")
         self._positions(p, B, key_pos, query_pos, mass)
         p.workspace_bytes = n = self._bytes[0 if mass is None else 1]
-        p.workspace, stream = self._scratch("attention", n)
-        self._call("pqhsa_paged_attention", self._ref, stream)
+        scratch, stream, capturing = self._scratch("attention")
+        with scratch.lock:
+            p.workspace = scratch.take(n, self.device, True, capturing)
+            self._call("pqhsa_paged_attention", self._ref, stream)
         return out
 
     def append(self, keys: torch.Tensor, values: torch.Tensor, seq_lens: torch.Tensor, *, new_lens: torch.Tensor | None = None,
@@ -364,13 +369,12 @@ class PagedAttention:
         nm = p.mass if new_mass is None else self._per_slot(new_mass, "new_mass", torch.float32, B)
         npos = p.key_pos if new_pos is None else self._per_slot(new_pos, "new_pos", torch.int32, B)
         n = 4 * B * self.H * (2 * budget + 8)
-        scratch, stream = self._scratch("evict", n + 4 * B * self.H * budget)
-        if source is None:
-            src = scratch + n
-        else:
-            if (source.dtype is not torch.int32 or source.get_device() != self._index or source.shape != (B, self.H, budget)
-                    or not source.is_contiguous()):
-                raise ValueError(f"source must be a contiguous int32 [{B}, {self.H}, {budget}] tensor on {self.device}")
-            src = source.data_ptr()
-        self._call("pqhsa_paged_evict", self._evict_ref, int(budget), int(recent), to, nm, npos, src, scratch, stream)
+        if source is not None and (source.dtype is not torch.int32 or source.get_device() != self._index
+                                   or source.shape != (B, self.H, budget) or not source.is_contiguous()):
+            raise ValueError(f"source must be a contiguous int32 [{B}, {self.H}, {budget}] tensor on {self.device}")
+        scratch, stream, capturing = self._scratch("evict")
+        with scratch.lock:
+            lists = scratch.take(n + 4 * B * self.H * budget, self.device, False, capturing)
+            src = lists + n if source is None else source.data_ptr()
+            self._call("pqhsa_paged_evict", self._evict_ref, int(budget), int(recent), to, nm, npos, src, lists, stream)
         return seq_lens if new_lens is None else new_lens

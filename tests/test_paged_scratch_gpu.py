@@ -123,7 +123,7 @@ def test_the_layers_of_a_model_share_their_scratch():
         check(o, None, w)
 
 
-def test_two_threads_on_one_stream_do_not_share():
+def test_two_threads_on_one_stream():
     """An attention with weights is two kernels; another thread's call on the same stream can come between them."""
     H, G = 2, 4
     caches = [Cache([2000, 300], H, BF, 16, "heads", seed=s) for s in (1, 2)]
@@ -152,3 +152,28 @@ def test_two_threads_on_one_stream_do_not_share():
         for _ in range(200):
             total += one
         assert torch.equal(m, total)
+
+
+def test_threads_that_come_and_go_leave_nothing_behind():
+    cache = Cache([300, 77], 2, BF, 16, "heads")
+    q, want = queries(cache, 4, 1), ref.attend(cache, queries(cache, 4, 1))
+    att, out = layer(cache, 4), torch.empty_like(q)
+    att.forward(q, cache.seq_lens, out=out)
+    gate = threading.Barrier(12)
+
+    def work():
+        gate.wait()  # all alive at once: no thread takes over another's identity
+        with turn:
+            att.forward(q, cache.seq_lens, out=out)
+
+    turn = threading.Lock()
+
+    def all_of_them():
+        threads = [threading.Thread(target=work) for _ in range(12)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+
+    assert grown(all_of_them)[0] == 0
+    check(out, None, want)
