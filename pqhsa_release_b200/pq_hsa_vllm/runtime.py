@@ -360,7 +360,7 @@ def should_dense_decode(impl, kv_cache, attn_metadata, extra=()) -> bool:
         return reject("dense_heads")
     if kv_cache.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         return reject("dense_dtype")
-    if T > 1 and getattr(attn_metadata, "causal", True) is False:  # tokens drafted in parallel see each other; of one token both are the same
+    if T > 1 and not getattr(attn_metadata, "causal", True):  # tokens drafted in parallel see each other; of one token both are the same
         return reject("dense_not_causal")
     left, right = tuple(getattr(impl, "sliding_window", None) or (-1, -1))
     if right > 0 or getattr(impl, "sinks", None) is not None or getattr(impl, "kv_sharing_target_layer_name", None) is not None:
